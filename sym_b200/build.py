@@ -16,11 +16,13 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 LIB_DIR = PKG / "_lib"
+OBJ_DIR = PKG / "_build"
 CUDA_SOURCES = sorted((PKG / "csrc" / "cuda").glob("*.cu"))
 RUNTIME_SOURCES = sorted((PKG / "csrc" / "runtime").glob("*.cpp"))
 HEADERS = (sorted((ROOT / "include").rglob("*.h")) + sorted((PKG / "csrc").rglob("*.hpp"))
@@ -54,6 +56,15 @@ def _stale(target: Path, sources) -> bool:
     return any(s.stat().st_mtime > t for s in sources)
 
 
+def _dependencies(listing: Path, default):
+    """This repository's files in a compiler's dependency listing."""
+    if not listing.exists():
+        return default
+    named = [Path(w) for w in listing.read_text().replace("\\\n", " ").split(":", 1)[-1].split()]
+    ours = [p for p in named if ROOT in p.resolve().parents]
+    return ours if ours and all(p.exists() for p in ours) else default
+
+
 def _run(cmd, verbose):
     if verbose:
         print(" ".join(str(c) for c in cmd), flush=True)
@@ -66,9 +77,25 @@ def build(force: bool = False, verbose: bool = False) -> None:
     if force or _stale(CUDA_LIB, CUDA_SOURCES + HEADERS):
         # SYM_B200_NVCC_DEFINES: extra -D tuning definitions (e.g. "SBC_TMA_STAGES=8")
         defines = [f"-D{d}" for d in os.environ.get("SYM_B200_NVCC_DEFINES", "").split() if d]
-        cmd = [_nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "--shared", "-Xcompiler", "-fPIC",
-               "-ccbin", _cxx(), *defines, *inc, *CUDA_SOURCES, "-o", CUDA_LIB]
-        _run(cmd, verbose)
+        cmd = [_nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-ccbin", _cxx(), *defines,
+               *inc]
+        # One object per source, compiled in parallel; an object is kept while
+        # the files its dependency list names are older and it was made with
+        # the same command line (recorded beside it).
+        OBJ_DIR.mkdir(exist_ok=True)
+        recipe = OBJ_DIR / "command"
+        line = " ".join(str(c) for c in cmd)
+        same = recipe.exists() and recipe.read_text() == line
+        objects, todo = [], []
+        for src in CUDA_SOURCES:
+            obj = OBJ_DIR / (src.stem + ".o")
+            objects.append(obj)
+            if force or not same or _stale(obj, _dependencies(obj.with_suffix(".d"), [src] + HEADERS)):
+                todo.append([*cmd, "-MD", "-MF", obj.with_suffix(".d"), "-c", src, "-o", obj])
+        with ThreadPoolExecutor(max_workers=max(1, min(len(todo), os.cpu_count() or 1))) as pool:
+            list(pool.map(lambda c: _run(c, verbose), todo))
+        recipe.write_text(line)
+        _run([_nvcc(), *ARCH, "--shared", "-ccbin", _cxx(), *objects, "-o", CUDA_LIB], verbose)
     if force or _stale(RUNTIME_LIB, RUNTIME_SOURCES + HEADERS + [CUDA_LIB]):
         cmd = [_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off", "-fno-fast-math",
                "-Wall", "-Wextra", "-Wno-unused-parameter", *inc, "-I", PKG / "csrc" / "runtime",

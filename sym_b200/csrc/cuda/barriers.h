@@ -1,0 +1,70 @@
+// sym_b200 -- shared-memory barriers with bounded waits, and the tensor map
+// encoder: what every kernel that is fed by asynchronous copies uses.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <cstdint>
+
+namespace sbc {
+
+/// Launch counters and the wait limit of this library (defined in
+/// relocate.cu; sbc_launch_count, sbc_wait_launch_count,
+/// sbc_set_wait_limit_ns).
+void count_launch();
+void count_wait_launch();
+uint64_t wait_limit_ns();
+
+/// cuTensorMapEncodeTiled of the loaded driver, or NULL.
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes)
+               : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+__device__ __forceinline__ uint64_t global_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+
+__device__ __forceinline__ bool mbar_try(uint32_t a, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+               " selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(done)
+               : "r"(a), "r"(parity)
+               : "memory");
+  return done != 0;
+}
+
+/// Wait for `parity` for at most `limit_ns` of the global timer (read only
+/// once the first poll failed); true when the phase completed.
+__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint64_t limit_ns) {
+  const uint32_t a = smem_addr(bar);
+  if (mbar_try(a, parity))
+    return true;
+  const uint64_t t0 = global_ns();
+  for (;;) {
+    if (mbar_try(a, parity))
+      return true;
+    if (global_ns() - t0 > limit_ns)
+      return false;
+  }
+}
+
+} // namespace sbc

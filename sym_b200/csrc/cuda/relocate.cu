@@ -15,6 +15,8 @@
 // outputs are bit-identical to the reference CPU executor for every input.
 #include "sb_cuda.h"
 
+#include "barriers.h"
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -26,6 +28,8 @@
 #include <mutex>
 
 namespace {
+
+using namespace sbc;
 
 std::atomic<uint64_t> g_launches{0};
 // Launches of kernels with bounded waits (the only writers of a descriptor's
@@ -1240,19 +1244,6 @@ constexpr int KTmaTileBytes = 64 * 128;
 constexpr int KTmaConsumers = 256;              // warps 0-7
 constexpr int KTmaThreads = KTmaConsumers + 32; // + the producer warp
 
-__device__ __forceinline__ uint32_t smem_addr(const void *p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void mbar_init(uint64_t *bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes)
-               : "memory");
-}
-
 /// Job order of k_tma_tile. Jobs walk groups of 2^lg source-column blocks (of
 /// 128 bytes); inside a group the column block varies fastest, so the tiles
 /// in flight at once read 2^lg * 128 contiguous bytes of each source row
@@ -1274,10 +1265,6 @@ __device__ __forceinline__ void tile_of(uint32_t job, const TileOrder &o, uint32
 /// groups 8c..8c+3 or 8c+4..8c+7, c = 0..7) fall on 32 distinct banks.
 __device__ __forceinline__ int param_slot(int n) { return n ^ (((n >> 5) & 1) << 2); }
 
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
 /// Raise the phase's expected transaction bytes without arriving.
 __device__ __forceinline__ void mbar_expect_tx_only(uint64_t *bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes)
@@ -1295,37 +1282,6 @@ __device__ __forceinline__ void cp_async4(void *dst_smem, const void *src_global
 /// completed (the barrier's expected count includes it: no increment).
 __device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
-__device__ __forceinline__ uint64_t global_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-__device__ __forceinline__ bool mbar_try(uint32_t a, uint32_t parity) {
-  uint32_t done;
-  asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-               " selp.u32 %0, 1, 0, p;\n}"
-               : "=r"(done)
-               : "r"(a), "r"(parity)
-               : "memory");
-  return done != 0;
-}
-
-/// Wait for `parity` for at most `limit_ns` of the global timer (read only
-/// once the first poll failed); true when the phase completed.
-__device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint64_t limit_ns) {
-  const uint32_t a = smem_addr(bar);
-  if (mbar_try(a, parity))
-    return true;
-  const uint64_t t0 = global_ns();
-  for (;;) {
-    if (mbar_try(a, parity))
-      return true;
-    if (global_ns() - t0 > limit_ns)
-      return false;
-  }
 }
 
 // Cache-policy tuning points of k_tma_tile: SBC_TMA_LOAD_EVICT_FIRST = 1
@@ -2178,21 +2134,6 @@ uint32_t tma_group_log2() {
   return lg;
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    else
-      cudaGetLastError();
-  });
-  return fn;
-}
-
 /// The 3-D view of a [rows, cols] box of `ws`-byte cells used by k_tma_tile:
 /// x = column (128 bytes of cells per box), y = group of `gr` rows (stride
 /// gr*pitch), z = row in group (stride pitch); box (128 / ws) x (64 / gr) x gr
@@ -2510,6 +2451,29 @@ int launch_tma(const sbc_relocate &d, int chain, int ch_on, const void *const *b
 }
 
 } // namespace
+
+namespace sbc {
+
+void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+void count_wait_launch() { g_wait_launches.fetch_add(1, std::memory_order_relaxed); }
+uint64_t wait_limit_ns() { return g_wait_ns.load(std::memory_order_relaxed); }
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    else
+      cudaGetLastError();
+  });
+  return fn;
+}
+
+} // namespace sbc
 
 extern "C" {
 
