@@ -167,6 +167,52 @@ void sbc_set_wait_limit_ns(uint64_t ns);
 int sbc_test_fault_mode(int mode);
 void sbc_test_withhold_tile(uint32_t job, uint64_t wait_limit_ns);
 
+/* ---- microscaled matrices (formats and layouts: csrc/cuda/mx_values.h) --- */
+enum sbc_dtype { SBC_F32 = 0, SBC_F16 = 1, SBC_BF16 = 2 };
+enum sbc_mx_format { SBC_MXFP4 = 0, SBC_MXINT8 = 1 };
+
+/* A matrix [rows, cols] in blocks of 32 columns with one power-of-two scale
+ * each. codes: 16 (mxfp4) or 32 (mxint8) bytes per block, rows padded to whole
+ * blocks. scales: mxfp4 512 bytes per 128 rows x 4 blocks; mxint8 one byte
+ * per block, row-major. Device memory, 16-byte aligned. */
+typedef struct {
+  void *codes;
+  void *scales;
+  int64_t rows;
+  int64_t cols;
+  int32_t format; /* sbc_mx_format */
+  int32_t reserved;
+} sbc_mx;
+
+/* x [rows, cols] (sbc_dtype, rows `row_stride` elements apart) to `along`
+ * (blocks along the columns) and / or `across` (mxfp4 [cols, rows]: blocks
+ * along the rows), either may be NULL. Also sets `clear_words` words at
+ * `clear` (or NULL) to zero. */
+int sbc_mx_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols, int64_t row_stride, const sbc_mx *along,
+                    const sbc_mx *across, uint32_t *clear, int64_t clear_words, void *stream);
+/* The values of q to `out`: dense [rows, cols], or [cols, rows] with
+ * `transpose` (mxfp4). */
+int sbc_mx_dequantize(const sbc_mx *q, void *out, int32_t dtype, int32_t transpose, void *stream);
+/* y [m, n] = a [m, k] b [n, k]^T, both mxfp4. `workspace`: device memory of
+ * the size given by sbc_mx_product_workspace, 256-byte aligned, whose first
+ * sbc_mx_product_clear_words words the call sets to zero, or with
+ * after_quantize the sbc_mx_quantize launch directly before it on `stream`,
+ * whose end the product then overlaps. */
+int sbc_mx_product_workspace(int64_t m, int64_t n, int64_t k, int64_t *bytes);
+int64_t sbc_mx_product_clear_words(int64_t m, int64_t n, int64_t k);
+int sbc_mx_product(const sbc_mx *a, const sbc_mx *b, void *y, int32_t dtype, void *workspace, int32_t after_quantize,
+                   void *stream);
+/* 2 once after a product whose bounded wait ran out (its output is
+ * incomplete), else 0; -1 when the word could not be allocated. */
+int sbc_mx_take_fault(void);
+/* h = silu(gate) up over [rows, cols]; gate_q, up_q (mxint8, or both NULL)
+ * keep the inputs in 8 bits. Rows are `*_stride` elements apart; h is dense. */
+int sbc_silu_mul(const void *gate, int64_t gate_stride, const void *up, int64_t up_stride, int32_t dtype, int64_t rows,
+                 int64_t cols, void *h, const sbc_mx *gate_q, const sbc_mx *up_q, void *stream);
+/* Its gradients from the 8-bit inputs. */
+int sbc_silu_mul_backward(const void *dh, int64_t dh_stride, int32_t dtype, const sbc_mx *gate_q, const sbc_mx *up_q,
+                          void *dgate, int64_t dgate_stride, void *dup, int64_t dup_stride, void *stream);
+
 /* ---- devices, memory and copies */
 int sbc_device_count(int *count);
 int sbc_set_device(int device);

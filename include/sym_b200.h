@@ -242,6 +242,66 @@ int sb_resources_clear(sb_resources *resources, sb_error *err);
 int sb_resources_close(sb_resources *resources, sb_error *err);
 void sb_resources_free(sb_resources *resources);
 
+/* ---- microscaled matrices (no reference counterpart) ----------------------
+ * Blocks of 32 values of a row share one power-of-two scale 2^s, held as the
+ * byte s + 127; byte 255 marks a block that held an infinity or a NaN and
+ * stands for NaN. With e = floor(log2 of the block's largest magnitude):
+ *   mxfp4 (0)   s = max(e - 2, -127); 4-bit floats 0, .5, 1, 1.5, 2, 3, 4, 6
+ *               with a sign (bit 3), rounded to nearest, ties to even, at most 6.
+ *               codes: 16 bytes per block, the lower index in the lower half of
+ *               a byte. scales: tiles of 128 rows x 4 blocks, 512 bytes, the
+ *               tiles of 128 rows consecutive; row r, block b of a tile at byte
+ *               16 (r mod 32) + 4 (r / 32) + b; absent blocks of a row's last
+ *               tile hold 0.
+ *   mxint8 (1)  s = max(e, -120); k = rne(x 2^(6-s)), |k| <= 127.
+ *               codes: 32 bytes per block; scales: row-major.
+ * Rows are padded to whole blocks with zero codes. Codes and scales are device
+ * memory on 16-byte boundaries.
+ *
+ * dtype of values: 0 float32, 1 float16, 2 bfloat16; strides in elements,
+ * columns adjacent. All calls are asynchronous on `stream` (a cudaStream_t of
+ * the matrices' device), may be captured into a CUDA graph and leave the
+ * caller's device current. A product whose bounded wait ran out (no such wait
+ * runs out unless the device stalls for a second) is reported by the next
+ * product as backend_failure. */
+typedef struct {
+  uint64_t codes;
+  uint64_t scales;
+  int64_t rows;
+  int64_t cols;
+  int32_t format;
+  int32_t device;
+} sb_mx;
+
+/* x [rows, cols] to `along` [rows, cols] (blocks along the columns) and / or
+ * `across` (mxfp4 [cols, rows]: blocks along the rows) with one read of x;
+ * either may be NULL. */
+int sb_mx_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols, int64_t row_stride, const sb_mx *along,
+                   const sb_mx *across, void *stream, sb_error *err);
+/* The values of q: dense [rows, cols], or [cols, rows] with `transpose`
+ * (mxfp4 only). Each value is rounded once, to dtype. */
+int sb_mx_dequantize(const sb_mx *q, void *out, int32_t dtype, int32_t transpose, void *stream, sb_error *err);
+/* Bytes of workspace of an [m, k] x [n, k] product on `device`; `quantize`:
+ * of sb_mx_linear. A workspace (256-byte aligned) belongs to one call at a
+ * time: calls that may overlap need one each. */
+int sb_mx_workspace(int64_t m, int64_t n, int64_t k, int32_t quantize, int32_t device, int64_t *bytes, sb_error *err);
+/* y [m, n] = a [m, k] b [n, k]^T (both mxfp4), dense. */
+int sb_mx_matmul(const sb_mx *a, const sb_mx *b, void *y, int32_t dtype, void *workspace, int64_t workspace_bytes,
+                 void *stream, sb_error *err);
+/* The same with a = the mxfp4 form of x [rows, k], made in the call. */
+int sb_mx_linear(const void *x, int32_t x_dtype, int64_t rows, int64_t row_stride, const sb_mx *weight, void *y,
+                 int32_t y_dtype, void *workspace, int64_t workspace_bytes, void *stream, sb_error *err);
+/* h [rows, cols] = silu(gate) up, dense; gate_q, up_q (mxint8, or both NULL)
+ * keep the inputs for the backward call. */
+int sb_silu_mul(const void *gate, int64_t gate_stride, const void *up, int64_t up_stride, int32_t dtype, int64_t rows,
+                int64_t cols, int32_t device, void *h, const sb_mx *gate_q, const sb_mx *up_q, void *stream,
+                sb_error *err);
+/* dgate = dh u s (1 + g (1 - s)), dup = dh g s with s = 1 / (1 + exp(-g)) and
+ * g, u as the kept inputs stand for them. */
+int sb_silu_mul_backward(const void *dh, int64_t dh_stride, int32_t dtype, const sb_mx *gate_q, const sb_mx *up_q,
+                         void *dgate, int64_t dgate_stride, void *dup, int64_t dup_stride, void *stream,
+                         sb_error *err);
+
 #ifdef __cplusplus
 }
 #endif

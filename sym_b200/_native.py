@@ -43,6 +43,11 @@ class SbGroupEntry(ctypes.Structure):
     _fields_ = [("plan", ctypes.c_void_p), ("source", SbView), ("destination", SbView), ("direction", ctypes.c_int32)]
 
 
+class SbMx(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_uint64), ("scales", ctypes.c_uint64), ("rows", ctypes.c_int64),
+                ("cols", ctypes.c_int64), ("format", ctypes.c_int32), ("device", ctypes.c_int32)]
+
+
 ROUTES = {"auto": 0, "dma_ring": 1, "zero_copy": 2, "staged": 3}
 
 _lib = None
@@ -59,6 +64,7 @@ def lib():
     L = ctypes.CDLL(str(RUNTIME_LIB))
     vp, sz, i32, i64, u64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint64
     ep = ctypes.POINTER(SbError)
+    mp = ctypes.POINTER(SbMx)
     cpp = ctypes.POINTER(ctypes.c_char_p)
     pp = ctypes.POINTER(ctypes.c_void_p)
     sig = {
@@ -109,6 +115,13 @@ def lib():
         "sb_completion_query": (ctypes.c_int, [vp, ctypes.POINTER(i32), ep]),
         "sb_completion_wait_stream": (ctypes.c_int, [vp, vp, ep]),
         "sb_completion_free": (None, [vp]),
+        "sb_mx_quantize": (ctypes.c_int, [vp, i32, i64, i64, i64, mp, mp, vp, ep]),
+        "sb_mx_dequantize": (ctypes.c_int, [mp, vp, i32, i32, vp, ep]),
+        "sb_mx_workspace": (ctypes.c_int, [i64, i64, i64, i32, i32, ctypes.POINTER(i64), ep]),
+        "sb_mx_matmul": (ctypes.c_int, [mp, mp, vp, i32, vp, i64, vp, ep]),
+        "sb_mx_linear": (ctypes.c_int, [vp, i32, i64, i64, mp, vp, i32, vp, i64, vp, ep]),
+        "sb_silu_mul": (ctypes.c_int, [vp, i64, vp, i64, i32, i64, i64, i32, vp, mp, mp, vp, ep]),
+        "sb_silu_mul_backward": (ctypes.c_int, [vp, i64, i32, mp, mp, vp, i64, vp, i64, vp, ep]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -1,0 +1,430 @@
+"""Microscaled matrices: 4-bit weights and products, 8-bit activation checkpoints.
+
+A row is cut into blocks of 32 values that share one power-of-two scale. Two
+formats (exact definitions: the last section of ``include/sym_b200.h``):
+
+``mxfp4``
+    4-bit floating point (0, .5, 1, 1.5, 2, 3, 4, 6 with a sign), 4.25 bits per
+    value: weights, and the operands of products on the tensor cores.
+``mxint8``
+    8-bit integers, 8.25 bits per value: activations kept for a backward pass.
+
+They stand beside the int8 paths of this package: ``workloads.WeightFetcher``
+expands int8 weights to ``[in, out]`` values, ``dequantize(w, transpose=True)``
+does so for mxfp4 weights, and ``linear`` multiplies with them directly.
+
+``quantize`` / ``quantize_both``   values -> codes, along the last axis or the first
+``dequantize``                     codes -> values, in their layout or transposed
+``matmul``                         product of two mxfp4 matrices
+``linear``                         values times an mxfp4 weight (serving), or times a
+                                   float weight with all three products of a training
+                                   step on mxfp4 operands
+``silu_mul``                       silu(gate) * up, keeping gate and up in 8 bits for
+                                   the backward pass
+
+All calls run on the current stream of the tensors' device, allocate from
+torch's caching allocator only and can be captured into CUDA graphs (a backward
+pass, as torch asks, only while no eager graph of the same leaves is alive).
+They have no CPU execution. Wrong arguments raise ``ValueError`` or ``TypeError``; failures of the
+native layer raise ``pyreloc.TransferError``.
+"""
+from __future__ import annotations
+
+import ctypes
+import threading
+from functools import lru_cache
+
+import torch
+
+from . import _native
+from .pyreloc import _raise_transfer
+
+BLOCK = 32
+FORMATS = {"mxfp4": 0, "mxint8": 1}
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_CODE_BYTES = {"mxfp4": 16, "mxint8": 32}  # per block
+
+
+class _Scratch(threading.local):
+    def __init__(self):
+        self.error = _native.SbError()
+        self.ref = ctypes.byref(self.error)
+
+
+_scratch = _Scratch()
+
+
+def _check(rc):
+    if rc:
+        _raise_transfer(_scratch.error)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _blocks(cols):
+    return -(-cols // BLOCK)
+
+
+def _scale_bytes(rows, cols, format):
+    if format == "mxfp4":
+        return -(-rows // 128) * -(-cols // 128) * 512
+    return rows * _blocks(cols)
+
+
+class MxTensor:
+    """A microscaled matrix ``[rows, cols]``: uint8 ``codes`` ``[rows, bytes]``
+    and uint8 ``scales`` (flat, in the format's order).
+
+    The constructor takes tensors that already have that layout, without a
+    copy; ``from_rows`` takes row-major scales, as checkpoints hold them."""
+
+    __slots__ = ("codes", "scales", "shape", "format", "native")
+
+    def __init__(self, codes, scales, shape, format="mxfp4"):
+        if format not in FORMATS:
+            raise ValueError(f"format must be one of {sorted(FORMATS)}")
+        rows, cols = shape
+        if rows < 0 or cols < 1:
+            raise ValueError("a microscaled matrix has at least one column")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("codes and scales are uint8 tensors")
+        if codes.device != scales.device:
+            raise ValueError("codes and scales live on different devices")
+        if tuple(codes.shape) != (rows, _blocks(cols) * _CODE_BYTES[format]) or not codes.is_contiguous():
+            raise ValueError(f"{format} codes of [{rows}, {cols}] are a contiguous "
+                             f"[{rows}, {_blocks(cols) * _CODE_BYTES[format]}] tensor")
+        if scales.numel() != _scale_bytes(rows, cols, format) or not scales.is_contiguous():
+            raise ValueError(f"{format} scales of [{rows}, {cols}] are {_scale_bytes(rows, cols, format)} "
+                             "contiguous bytes")
+        self.codes, self.scales, self.shape, self.format = codes, scales, (rows, cols), format
+        self.native = None
+        if codes.is_cuda and rows:
+            if codes.data_ptr() % 16 or scales.data_ptr() % 16:
+                raise ValueError("codes and scales start on 16-byte boundaries")
+            self.native = _native.SbMx(codes.data_ptr(), scales.data_ptr(), rows, cols, FORMATS[format],
+                                       codes.device.index)
+
+    @classmethod
+    def empty(cls, rows, cols, device, format="mxfp4"):
+        codes = torch.empty((rows, _blocks(cols) * _CODE_BYTES[format]), dtype=torch.uint8, device=device)
+        scales = torch.empty(_scale_bytes(rows, cols, format), dtype=torch.uint8, device=device)
+        return cls(codes, scales, (rows, cols), format)
+
+    @classmethod
+    def from_rows(cls, codes, row_scales, cols, format="mxfp4"):
+        """From codes and row-major scales ``[rows, blocks]``."""
+        rows, blocks = row_scales.shape
+        if blocks != _blocks(cols):
+            raise ValueError(f"rows of {cols} values have {_blocks(cols)} scales")
+        if format == "mxfp4":
+            tiles = torch.nn.functional.pad(row_scales, (0, -blocks % 4, 0, -rows % 128))
+            row_scales = tiles.view(-(-rows // 128), 4, 32, -(-blocks // 4), 4).permute(0, 3, 2, 1, 4)
+        return cls(codes.contiguous(), row_scales.contiguous().flatten(), (rows, cols), format)
+
+    def row_scales(self):
+        """The scale bytes, row-major ``[rows, blocks]``."""
+        rows, cols = self.shape
+        blocks = _blocks(cols)
+        if self.format == "mxint8":
+            return self.scales.view(rows, blocks)
+        tiles = self.scales.view(-(-rows // 128), -(-blocks // 4), 32, 4, 4).permute(0, 3, 2, 1, 4)
+        return tiles.reshape(-(-rows // 128) * 128, -(-blocks // 4) * 4)[:rows, :blocks].contiguous()
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def to(self, device, non_blocking=False):
+        return MxTensor(self.codes.to(device, non_blocking=non_blocking),
+                        self.scales.to(device, non_blocking=non_blocking), self.shape, self.format)
+
+    def __repr__(self):
+        return f"MxTensor({list(self.shape)}, {self.format}, {self.device})"
+
+
+def _matrix(x, name):
+    """x as a matrix whose columns are adjacent: (tensor, rows, cols, row stride)."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    rows, cols = x.shape
+    if cols > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    return x, rows, cols, x.stride(0) if rows > 1 else cols
+
+
+def _values(x, name, least=1):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} is a tensor")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"{name} is float32, float16 or bfloat16")
+    if not x.is_cuda:
+        raise ValueError(f"{name} is on {x.device}: microscaled operators run on CUDA devices")
+    if x.dim() < least or x.shape[-1] == 0:
+        raise ValueError(f"{name} needs {'rows and columns' if least == 2 else 'at least one column'}")
+    return x
+
+
+def _mx(q, name, format=None):
+    if not isinstance(q, MxTensor):
+        raise TypeError(f"{name} is an MxTensor")
+    if not q.codes.is_cuda:
+        raise ValueError(f"{name} is on {q.device}: microscaled operators run on CUDA devices")
+    if format is not None and q.format != format:
+        raise ValueError(f"{name} is {q.format}: {format} is needed")
+    return q
+
+
+def _result(dtype, default):
+    dtype = default if dtype is None else dtype
+    if dtype not in _DTYPES:
+        raise TypeError("results are float32, float16 or bfloat16")
+    return dtype
+
+
+def _quantize(x, format, along, across):
+    x, rows, cols, stride = _matrix(x, "x")
+    q = MxTensor.empty(rows, cols, x.device, format) if along else None
+    qt = MxTensor.empty(cols, rows, x.device) if across else None
+    if rows:
+        _check(_native.lib().sb_mx_quantize(
+            x.data_ptr(), _DTYPES[x.dtype], rows, cols, stride, q.native if along else None,
+            qt.native if across else None, _stream(x.device), _scratch.ref))
+    return q, qt
+
+
+def quantize(x, format="mxfp4", *, along=-1):
+    """Values ``[..., cols]`` to an ``MxTensor`` ``[rows, cols]`` whose blocks run
+    along the last axis (leading axes are flattened), or for a matrix with
+    ``along=0`` to the mxfp4 form of its transpose, whose blocks run along
+    the first axis."""
+    _values(x, "x")
+    if format not in FORMATS:
+        raise ValueError(f"format must be one of {sorted(FORMATS)}")
+    if along not in (0, -1):
+        raise ValueError("along must be -1 or 0")
+    x = x.detach()
+    if along == 0:
+        if x.dim() != 2 or x.shape[0] == 0:
+            raise ValueError("along=0 takes a matrix with at least one row")
+        if format != "mxfp4":
+            raise ValueError("along=0 is defined for mxfp4")
+    if x.dim() == 2 and format == "mxfp4" and x.shape[0] > 1 and x.shape[1] > 1 and x.stride(0) == 1 != x.stride(1):
+        # a transposed view: the other direction of the matrix behind it
+        return _quantize(x.t(), format, along == 0, along != 0)[0 if along == 0 else 1]
+    q, qt = _quantize(x, format, along != 0, along == 0)
+    return q if qt is None else qt
+
+
+def quantize_both(x):
+    """A matrix's two mxfp4 forms with one read of it: ``(quantize(x),
+    quantize(x, along=0))``, what a training step's products take."""
+    if _values(x, "x").dim() != 2 or x.shape[0] == 0:
+        raise ValueError("quantize_both takes a matrix with at least one row")
+    return _quantize(x.detach(), "mxfp4", True, True)
+
+
+def dequantize(q, dtype=torch.float16, *, transpose=False):
+    """The values of an ``MxTensor``, each rounded once to ``dtype``: ``[rows,
+    cols]``, or ``[cols, rows]`` with ``transpose`` (mxfp4), the layout that a
+    product ``x @ w`` takes."""
+    _mx(q, "q")
+    dtype = _result(dtype, None)
+    if transpose and q.format != "mxfp4":
+        raise ValueError("transpose is defined for mxfp4")
+    rows, cols = q.shape
+    out = torch.empty((cols, rows) if transpose else (rows, cols), dtype=dtype, device=q.device)
+    if rows:
+        _check(_native.lib().sb_mx_dequantize(q.native, out.data_ptr(), _DTYPES[dtype], int(transpose),
+                                              _stream(q.device), _scratch.ref))
+    return out
+
+
+@lru_cache(maxsize=4096)
+def _workspace(m, n, k, quantize, device):
+    bytes_ = ctypes.c_int64()
+    _check(_native.lib().sb_mx_workspace(m, n, k, quantize, device, ctypes.byref(bytes_), _scratch.ref))
+    return bytes_.value
+
+
+def matmul(a, b, *, dtype=torch.bfloat16):
+    """``a [m, k]`` times the transpose of ``b [n, k]``, both mxfp4, accumulated in
+    32 bits and rounded once to ``dtype``."""
+    _mx(a, "a", "mxfp4"), _mx(b, "b", "mxfp4")
+    dtype = _result(dtype, None)
+    if a.device != b.device:
+        raise ValueError("a and b live on different devices")
+    (m, k), (n, kb) = a.shape, b.shape
+    if k != kb:
+        raise ValueError(f"a [m, k] and b [n, k] need the same k: got {k} and {kb}")
+    y = torch.empty((m, n), dtype=dtype, device=a.device)
+    if m and n:
+        size = _workspace(m, n, k, 0, a.device.index)
+        space = torch.empty(size, dtype=torch.uint8, device=a.device)
+        _check(_native.lib().sb_mx_matmul(a.native, b.native, y.data_ptr(), _DTYPES[dtype], space.data_ptr(), size,
+                                          _stream(a.device), _scratch.ref))
+    return y
+
+
+def _linear(x, w, dtype):
+    lead = x.shape[:-1]
+    x, m, k, stride = _matrix(x, "x")
+    n = w.shape[0]
+    y = torch.empty((*lead, n), dtype=dtype, device=x.device)
+    if m and n:
+        size = _workspace(m, n, k, 1, x.device.index)
+        space = torch.empty(size, dtype=torch.uint8, device=x.device)
+        _check(_native.lib().sb_mx_linear(x.data_ptr(), _DTYPES[x.dtype], m, stride, w.native, y.data_ptr(),
+                                          _DTYPES[dtype], space.data_ptr(), size, _stream(x.device), _scratch.ref))
+    return y
+
+
+class _FrozenLinear(torch.autograd.Function):
+    """A product with a 4-bit weight that is not trained."""
+
+    @staticmethod
+    def forward(ctx, x, w, wt, dtype):
+        ctx.save_for_backward(wt.codes, wt.scales)
+        ctx.shape, ctx.dtype = wt.shape, x.dtype
+        return _linear(x, w, dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return _linear(dy, MxTensor(*ctx.saved_tensors, ctx.shape), ctx.dtype), None, None, None
+
+
+class _TrainLinear(torch.autograd.Function):
+    """y = Q(x) Q(w)^T, dx = Q(dy) Q(w^T)^T, dw = Q(dy^T) Q(x^T)^T; every
+    tensor is read once for the forms that it is needed in, and what is kept
+    for the backward pass is kept in 4 bits."""
+
+    @staticmethod
+    def forward(ctx, x, weight, dtype):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        ctx.lead, ctx.dtypes = x.shape[:-1], (x.dtype, weight.dtype)
+        qx, qxt = _quantize(x, "mxfp4", True, need_w)
+        qw, qwt = _quantize(weight, "mxfp4", True, need_x)
+        kept = [q for q in (qxt, qwt) if q is not None]
+        ctx.shapes = [q.shape for q in kept]
+        ctx.save_for_backward(*(t for q in kept for t in (q.codes, q.scales)))
+        return matmul(qx, qw, dtype=dtype).view(*ctx.lead, weight.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        t = ctx.saved_tensors
+        kept = [MxTensor(t[2 * i], t[2 * i + 1], s) for i, s in enumerate(ctx.shapes)]
+        qdy, qdyt = _quantize(dy, "mxfp4", need_x, need_w)
+        dx = dw = None
+        if need_x:
+            dx = matmul(qdy, kept[-1], dtype=ctx.dtypes[0])
+            dx = dx.view(*ctx.lead, dx.shape[1])
+        if need_w:
+            dw = matmul(qdyt, kept[0], dtype=ctx.dtypes[1])
+        return dx, dw, None
+
+
+def linear(x, weight, weight_t=None, *, dtype=None):
+    """``x [..., k]`` times the transpose of ``weight [n, k]``, with both operands in
+    mxfp4 (blocks along k) and 32-bit accumulation; the result ``[..., n]`` has
+    ``dtype`` (default: that of x).
+
+    ``weight`` an ``MxTensor``: serving, any number of rows of x from one token
+    up. x is quantised in the call. Where x needs a gradient, pass
+    ``weight_t``, the mxfp4 form of the weight's transpose (``quantize_both``), for
+    ``dx = Q(dy) weight_t^T``.
+
+    ``weight`` a float tensor: training; x, weight and dy are quantised along the
+    axis that each product sums over, and the backward pass gives dx and dw."""
+    _values(x, "x")
+    dtype = _result(dtype, x.dtype)
+    if isinstance(weight, MxTensor):
+        _mx(weight, "weight", "mxfp4")
+    elif weight_t is not None:
+        raise ValueError("weight_t goes with an MxTensor weight")
+    elif _values(weight, "weight").dim() != 2:
+        raise ValueError("weight is a matrix [n, k]")
+    if weight.device != x.device:
+        raise ValueError("x and weight live on different devices")
+    n, k = weight.shape
+    if x.shape[-1] != k:
+        raise ValueError(f"x [..., k] and weight [n, k] need the same k: got {x.shape[-1]} and {k}")
+    if isinstance(weight, MxTensor):
+        if not (torch.is_grad_enabled() and x.requires_grad):
+            return _linear(x.detach(), weight, dtype)
+        if weight_t is None:
+            raise ValueError("x needs a gradient: pass weight_t, the mxfp4 form of the weight's transpose")
+        if _mx(weight_t, "weight_t", "mxfp4").shape != (k, n) or weight_t.device != x.device:
+            raise ValueError(f"weight_t is [{k}, {n}] on {x.device}")
+        return _FrozenLinear.apply(x, weight, weight_t, dtype)
+    if n == 0 or x.numel() == 0:
+        raise ValueError("a training product needs at least one row of x and of weight")
+    return _TrainLinear.apply(x, weight, dtype)
+
+
+class _SiluMul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, up):
+        ctx.packed = up is None
+        ctx.shape = gate.shape
+        parts = gate.chunk(2, -1) if up is None else (gate, up)
+        h, kept = _silu_mul(*parts, True)
+        ctx.save_for_backward(*(t for q in kept for t in (q.codes, q.scales)))
+        ctx.extents = kept[0].shape
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        t = ctx.saved_tensors
+        rows, cols = ctx.extents
+        dgate = torch.empty(ctx.shape, dtype=dh.dtype, device=dh.device)
+        dup = None if ctx.packed else torch.empty(ctx.shape, dtype=dh.dtype, device=dh.device)
+        if rows:
+            g, u = (MxTensor(t[i], t[i + 1], ctx.extents, "mxint8") for i in (0, 2))
+            dh, _, _, stride = _matrix(dh, "dh")
+            out = 2 * cols if ctx.packed else cols
+            at = dgate.data_ptr() + cols * dh.element_size() if ctx.packed else dup.data_ptr()
+            _check(_native.lib().sb_silu_mul_backward(
+                dh.data_ptr(), stride, _DTYPES[dh.dtype], g.native, u.native, dgate.data_ptr(), out, at, out,
+                _stream(dh.device), _scratch.ref))
+        return dgate, dup
+
+
+def _silu_mul(gate, up, keep):
+    lead = gate.shape
+    gate, rows, cols, gate_stride = _matrix(gate, "gate")
+    up, _, _, up_stride = _matrix(up, "up")
+    h = torch.empty(lead, dtype=gate.dtype, device=gate.device)
+    kept = [MxTensor.empty(rows, cols, gate.device, "mxint8") for _ in range(2)] if keep else [None, None]
+    if rows:
+        _check(_native.lib().sb_silu_mul(
+            gate.data_ptr(), gate_stride, up.data_ptr(), up_stride, _DTYPES[gate.dtype], rows, cols,
+            gate.device.index, h.data_ptr(), kept[0].native if keep else None, kept[1].native if keep else None,
+            _stream(gate.device), _scratch.ref))
+    return h, kept
+
+
+def silu_mul(gate, up=None):
+    """``silu(gate) * up`` elementwise, ``silu(g) = g / (1 + exp(-g))``; with ``up``
+    left out, ``gate`` holds both halves along its last axis.
+
+    Where a gradient is needed, gate and up are kept as mxint8 copies (8.25 bits
+    per value, step at most 2^-6 of the block's largest magnitude) instead of
+    as they are, and the backward pass computes both gradients from the copies.
+    The result itself is computed from the inputs."""
+    _values(gate, "gate")
+    if up is None:
+        if gate.shape[-1] % 2:
+            raise ValueError("gate and up in one tensor need an even last axis")
+    else:
+        _values(up, "up")
+        if up.shape != gate.shape or up.dtype != gate.dtype or up.device != gate.device:
+            raise ValueError("gate and up have the same shape, type and device")
+    if torch.is_grad_enabled() and (gate.requires_grad or (up is not None and up.requires_grad)):
+        return _SiluMul.apply(gate, up)
+    parts = gate.detach().chunk(2, -1) if up is None else (gate.detach(), up.detach())
+    return _silu_mul(*parts, False)[0]
