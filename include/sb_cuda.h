@@ -186,22 +186,20 @@ typedef struct {
 
 /* x [rows, cols] (sbc_dtype, rows `row_stride` elements apart) to `along`
  * (blocks along the columns) and / or `across` (mxfp4 [cols, rows]: blocks
- * along the rows), either may be NULL. Also sets `clear_words` words at
- * `clear` (or NULL) to zero. */
+ * along the rows), either may be NULL. */
 int sbc_mx_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols, int64_t row_stride, const sbc_mx *along,
-                    const sbc_mx *across, uint32_t *clear, int64_t clear_words, void *stream);
+                    const sbc_mx *across, void *stream);
 /* The values of q to `out`: dense [rows, cols], or [cols, rows] with
  * `transpose` (mxfp4). */
 int sbc_mx_dequantize(const sbc_mx *q, void *out, int32_t dtype, int32_t transpose, void *stream);
-/* y [m, n] = a [m, k] b [n, k]^T, both mxfp4. `workspace`: device memory of
- * the size given by sbc_mx_product_workspace, 256-byte aligned, whose first
- * sbc_mx_product_clear_words words the call sets to zero, or with
- * after_quantize the sbc_mx_quantize launch directly before it on `stream`,
- * whose end the product then overlaps. */
-int sbc_mx_product_workspace(int64_t m, int64_t n, int64_t k, int64_t *bytes);
-int64_t sbc_mx_product_clear_words(int64_t m, int64_t n, int64_t k);
-int sbc_mx_product(const sbc_mx *a, const sbc_mx *b, void *y, int32_t dtype, void *workspace, int32_t after_quantize,
-                   void *stream);
+/* y [m, n] = a [m, k] b [n, k]^T, both mxfp4. after_quantize: the launch
+ * directly before it on `stream` is the sbc_mx_quantize that writes a, whose
+ * end the product overlaps. Where sbc_mx_fuses_quantize(m, n, k) says so, a may
+ * be given as its values x [m, k] (x_dtype, rows x_stride elements apart)
+ * instead: `a` then has no codes and no scales. */
+int sbc_mx_fuses_quantize(int64_t m, int64_t n, int64_t k);
+int sbc_mx_product(const sbc_mx *a, const void *x, int32_t x_dtype, int64_t x_stride, const sbc_mx *b, void *y,
+                   int32_t dtype, int32_t after_quantize, void *stream);
 /* 2 once after a product whose bounded wait ran out (its output is
  * incomplete), else 0; -1 when the word could not be allocated. */
 int sbc_mx_take_fault(void);

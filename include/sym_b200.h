@@ -281,14 +281,13 @@ int sb_mx_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols, int
 /* The values of q: dense [rows, cols], or [cols, rows] with `transpose`
  * (mxfp4 only). Each value is rounded once, to dtype. */
 int sb_mx_dequantize(const sb_mx *q, void *out, int32_t dtype, int32_t transpose, void *stream, sb_error *err);
-/* Bytes of workspace of an [m, k] x [n, k] product on `device`; `quantize`:
- * of sb_mx_linear. A workspace (256-byte aligned) belongs to one call at a
- * time: calls that may overlap need one each. */
-int sb_mx_workspace(int64_t m, int64_t n, int64_t k, int32_t quantize, int32_t device, int64_t *bytes, sb_error *err);
 /* y [m, n] = a [m, k] b [n, k]^T (both mxfp4), dense. */
-int sb_mx_matmul(const sb_mx *a, const sb_mx *b, void *y, int32_t dtype, void *workspace, int64_t workspace_bytes,
-                 void *stream, sb_error *err);
-/* The same with a = the mxfp4 form of x [rows, k], made in the call. */
+int sb_mx_matmul(const sb_mx *a, const sb_mx *b, void *y, int32_t dtype, void *stream, sb_error *err);
+/* The same with a = the mxfp4 form of x [rows, k], made in the call. Its
+ * `workspace` (device memory, 256-byte aligned; sb_mx_linear_workspace bytes,
+ * none for a few rows) belongs to one call at a time: calls that may overlap
+ * need one each. */
+int sb_mx_linear_workspace(int64_t rows, int64_t n, int64_t k, int32_t device, int64_t *bytes, sb_error *err);
 int sb_mx_linear(const void *x, int32_t x_dtype, int64_t rows, int64_t row_stride, const sb_mx *weight, void *y,
                  int32_t y_dtype, void *workspace, int64_t workspace_bytes, void *stream, sb_error *err);
 /* h [rows, cols] = silu(gate) up, dense; gate_q, up_q (mxint8, or both NULL)

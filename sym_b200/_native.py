@@ -117,8 +117,8 @@ def lib():
         "sb_completion_free": (None, [vp]),
         "sb_mx_quantize": (ctypes.c_int, [vp, i32, i64, i64, i64, mp, mp, vp, ep]),
         "sb_mx_dequantize": (ctypes.c_int, [mp, vp, i32, i32, vp, ep]),
-        "sb_mx_workspace": (ctypes.c_int, [i64, i64, i64, i32, i32, ctypes.POINTER(i64), ep]),
-        "sb_mx_matmul": (ctypes.c_int, [mp, mp, vp, i32, vp, i64, vp, ep]),
+        "sb_mx_matmul": (ctypes.c_int, [mp, mp, vp, i32, vp, ep]),
+        "sb_mx_linear_workspace": (ctypes.c_int, [i64, i64, i64, i32, ctypes.POINTER(i64), ep]),
         "sb_mx_linear": (ctypes.c_int, [vp, i32, i64, i64, mp, vp, i32, vp, i64, vp, ep]),
         "sb_silu_mul": (ctypes.c_int, [vp, i64, vp, i64, i32, i64, i64, i32, vp, mp, mp, vp, ep]),
         "sb_silu_mul_backward": (ctypes.c_int, [vp, i64, i32, mp, mp, vp, i64, vp, i64, vp, ep]),

@@ -67,4 +67,22 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint64
   }
 }
 
+/// The same for kernels whose latency counts: the global timer is read only
+/// once in 64 failed polls, each of which sleeps for a while by itself.
+__device__ __forceinline__ bool mbar_wait_often(uint64_t *bar, uint32_t parity, uint64_t limit_ns) {
+  const uint32_t a = smem_addr(bar);
+  uint64_t t0 = 0;
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try(a, parity))
+        return true;
+    const uint64_t now = global_ns();
+    if (t0 == 0)
+      t0 = now;
+    else if (now - t0 > limit_ns)
+      return false;
+  }
+}
+
 } // namespace sbc

@@ -7,7 +7,8 @@
 //
 // Bound by memory: for 16-bit values the forward pass reads 4 bytes per
 // element and writes 2 + 2.06, the backward pass the same the other way
-// round. A thread takes 8 elements of one row, four lanes a block.
+// round. A block of threads takes 16 rows x 128 columns per unit, a thread 8
+// elements of a row, four lanes a block of 32.
 #include "barriers.h"
 #include "mx_values.h"
 
@@ -16,42 +17,51 @@ namespace {
 using namespace mx;
 
 constexpr int kThreads = 256;
-constexpr int kUnits = 2; // units of 8 elements per thread
+constexpr int kTile = 128;
+constexpr int kUnits = 2; // rows (16 apart) per thread
 
 struct GateArgs {
   const void *gate, *up; // forward: inputs; backward: `gate` is dh
   void *h, *dup;         // forward: h; backward: dgate (h) and dup
   int64_t gate_stride, up_stride, h_stride, dup_stride;
   uint8_t *gate_codes, *gate_scales, *up_codes, *up_scales;
-  int64_t rows, cols;
-  uint32_t row_units; // units of 8 per row, a multiple of 4
-  int64_t units;
+  int64_t rows, cols, blocks;
+  uint32_t tiles_c;
 };
 
 /// 1 / (1 + exp(-g)) from exp(-|g|), which cannot overflow: far below zero the
-/// result is exp(g), down to the subnormals.
-__device__ __forceinline__ float sigmoid(float g) {
-  const float e = expf(-fabsf(g));
-  return (g < 0.f ? e : 1.f) / (1.f + e);
+/// result is exp(g), down to the subnormals. For results in 16 bits the
+/// exponential is 2^(-|g| log2 e), log2 e as a sum of two 32-bit numbers so
+/// that one rounding of the exponent is left (|g| 2^-24 of the value), and the
+/// reciprocal of 1 .. 2 the hardware's (one unit in the last place): both
+/// thousands of times below a 16-bit step. 32-bit results take expf and an exact
+/// division.
+template <int DT> __device__ __forceinline__ float sigmoid(float g) {
+  const float a = -fabsf(g);
+  if (DT == SBC_F32) {
+    const float e = expf(a);
+    return (g < 0.f ? e : 1.f) / (1.f + e);
+  }
+  const float e = exp2f(fmaf(a, 1.44269502f, a * 1.92596303e-8f));
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return (g < 0.f ? e : 1.f) * r;
+}
+
+template <int DT> __device__ __forceinline__ float2 sigmoid2(float2 g) {
+  return make_float2(sigmoid<DT>(g.x), sigmoid<DT>(g.y));
 }
 
 /// Keep eight values of one block quarter in 8 bits.
-__device__ __forceinline__ void keep8(uint8_t *codes, uint8_t *scales, const float (&v)[8], int64_t block, int quarter,
-                                      bool in) {
-  float m = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    m = abs_max(m, v[i]);
-  m = abs_max(m, __shfl_xor_sync(~0u, m, 1));
-  m = abs_max(m, __shfl_xor_sync(~0u, m, 2));
-  const uint32_t byte = scale_byte<SBC_MXINT8>(m);
-  const float inv = inverse_scale<SBC_MXINT8>(byte);
-  uint2 w = make_uint2(codes8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-                       codes8x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+template <int DT>
+__device__ __forceinline__ void keep8(uint8_t *codes, uint8_t *scales, const Raw8<DT> &raw, const float2 (&v)[4],
+                                      int64_t block, int quarter, bool exists) {
+  const uint32_t byte = scale_byte<SBC_MXINT8>(top_of_lanes<2>(raw.top()));
+  uint2 w = codes8(v, inverse_scale<SBC_MXINT8>(byte));
   if (byte == 255)
     w = make_uint2(0, 0);
-  if (in) {
-    *reinterpret_cast<uint2 *>(codes + block * 32 + quarter * 8) = w;
+  if (exists) {
+    __stcs(reinterpret_cast<uint2 *>(codes + block * 32 + quarter * 8), w);
     if (quarter == 0)
       scales[block] = static_cast<uint8_t>(byte);
   }
@@ -60,23 +70,36 @@ __device__ __forceinline__ void keep8(uint8_t *codes, uint8_t *scales, const flo
 template <int DT, bool KEEP, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_silu_mul(const __grid_constant__ GateArgs a) {
   using T = typename Value<DT>::T;
+  const uint32_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x - tr * a.tiles_c;
+  const int64_t r0 = static_cast<int64_t>(tr) * (16 * kUnits) + (threadIdx.x >> 4);
+  const int64_t c = static_cast<int64_t>(tc) * kTile + (threadIdx.x & 15) * 8;
+  const int cols = static_cast<int>(a.cols - c < 0 ? 0 : a.cols - c < 8 ? a.cols - c : 8);
+  const T *gate_at = static_cast<const T *>(a.gate) + r0 * a.gate_stride + c;
+  const T *up_at = static_cast<const T *>(a.up) + r0 * a.up_stride + c;
+  T *h_at = static_cast<T *>(a.h) + r0 * a.cols + c;
+  const int64_t block = r0 * a.blocks + c / kBlock;
+  Raw8<DT> gate[kUnits], up[kUnits];
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kUnits + i) * kThreads + threadIdx.x;
-    const bool in = unit < a.units;
-    const int64_t r = in ? unit / a.row_units : 0, u8 = in ? unit - r * a.row_units : 0, c = u8 * 8;
-    const int have = !in ? 0 : static_cast<int>(a.cols - c < 0 ? 0 : a.cols - c < 8 ? a.cols - c : 8);
-    float g[8], u[8], h[8];
-    load8<DT, VEC>(g, static_cast<const T *>(a.gate) + r * a.gate_stride + c, have);
-    load8<DT, VEC>(u, static_cast<const T *>(a.up) + r * a.up_stride + c, have);
+    const int have = r0 + 16 * i < a.rows ? cols : 0;
+    gate[i].template load<VEC>(gate_at + 16 * i * a.gate_stride, have);
+    up[i].template load<VEC>(up_at + 16 * i * a.up_stride, have);
+  }
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      h[k] = g[k] * sigmoid(g[k]) * u[k];
-    store8<DT, VEC>(static_cast<T *>(a.h) + r * a.cols + c, h, have);
+  for (int i = 0; i < kUnits; ++i) {
+    float2 g[4], u[4], h[4];
+    gate[i].values(g);
+    up[i].values(u);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      h[k] = __fmul2_rn(__fmul2_rn(g[k], sigmoid2<DT>(g[k])), u[k]);
+    const bool row_exists = r0 + 16 * i < a.rows;
+    if (row_exists)
+      store8<DT, VEC>(h_at + 16 * i * a.cols, h, cols);
     if (KEEP) {
-      const int64_t block = r * (a.row_units / 4) + u8 / 4;
-      keep8(a.gate_codes, a.gate_scales, g, block, u8 & 3, in);
-      keep8(a.up_codes, a.up_scales, u, block, u8 & 3, in);
+      const bool exists = row_exists && c < a.blocks * kBlock;
+      keep8(a.gate_codes, a.gate_scales, gate[i], g, block + 16 * i * a.blocks, threadIdx.x & 3, exists);
+      keep8(a.up_codes, a.up_scales, up[i], u, block + 16 * i * a.blocks, threadIdx.x & 3, exists);
     }
   }
 }
@@ -84,32 +107,47 @@ __global__ void __launch_bounds__(kThreads) k_silu_mul(const __grid_constant__ G
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_silu_mul_backward(const __grid_constant__ GateArgs a) {
   using T = typename Value<DT>::T;
+  const uint32_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x - tr * a.tiles_c;
+  const int64_t r0 = static_cast<int64_t>(tr) * (16 * kUnits) + (threadIdx.x >> 4);
+  const int64_t c = static_cast<int64_t>(tc) * kTile + (threadIdx.x & 15) * 8;
+  const int cols = static_cast<int>(a.cols - c < 8 ? a.cols - c : 8);
+  if (cols <= 0)
+    return;
+  Raw8<DT> in[kUnits];
+  uint2 gate[kUnits], up[kUnits];
+  uint32_t gate_scale[kUnits], up_scale[kUnits];
+  const T *dh_at = static_cast<const T *>(a.gate) + r0 * a.gate_stride + c;
+  const int64_t block0 = r0 * a.blocks + c / kBlock;
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kUnits + i) * kThreads + threadIdx.x;
-    if (unit >= a.units)
-      return;
-    const int64_t r = unit / a.row_units, u8 = unit - r * a.row_units, c = u8 * 8;
-    const int have = static_cast<int>(a.cols - c < 0 ? 0 : a.cols - c < 8 ? a.cols - c : 8);
-    const int64_t block = r * (a.row_units / 4) + u8 / 4;
-    float dh[8], g[8], u[8], dg[8], du[8];
-    load8<DT, VEC>(dh, static_cast<const T *>(a.gate) + r * a.gate_stride + c, have);
-    const uint2 gw = __ldg(reinterpret_cast<const uint2 *>(a.gate_codes + block * 32 + (u8 & 3) * 8));
-    const uint2 uw = __ldg(reinterpret_cast<const uint2 *>(a.up_codes + block * 32 + (u8 & 3) * 8));
-    const float gs = scale_value<SBC_MXINT8>(__ldg(a.gate_scales + block));
-    const float us = scale_value<SBC_MXINT8>(__ldg(a.up_scales + block));
-    values8x4(g, gw.x);
-    values8x4(g + 4, gw.y);
-    values8x4(u, uw.x);
-    values8x4(u + 4, uw.y);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float gv = g[k] * gs, uv = u[k] * us, s = sigmoid(gv);
-      dg[k] = dh[k] * uv * (s * (1.f + gv * (1.f - s)));
-      du[k] = dh[k] * (gv * s);
+    const int64_t block = block0 + 16 * i * a.blocks, at = block * 32 + (threadIdx.x & 3) * 8;
+    if (r0 + 16 * i < a.rows) {
+      in[i].template load<VEC>(dh_at + 16 * i * a.gate_stride, cols);
+      gate[i] = __ldg(reinterpret_cast<const uint2 *>(a.gate_codes + at));
+      up[i] = __ldg(reinterpret_cast<const uint2 *>(a.up_codes + at));
+      gate_scale[i] = __ldg(a.gate_scales + block);
+      up_scale[i] = __ldg(a.up_scales + block);
     }
-    store8<DT, VEC>(static_cast<T *>(a.h) + r * a.h_stride + c, dg, have);
-    store8<DT, VEC>(static_cast<T *>(a.dup) + r * a.dup_stride + c, du, have);
+  }
+  T *dgate_at = static_cast<T *>(a.h) + r0 * a.h_stride + c, *dup_at = static_cast<T *>(a.dup) + r0 * a.dup_stride + c;
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    if (r0 + 16 * i >= a.rows)
+      return;
+    float2 dh[4], g[4], u[4], dg[4], du[4];
+    in[i].values(dh);
+    values8(g, gate[i], scale_value<SBC_MXINT8>(gate_scale[i]));
+    values8(u, up[i], scale_value<SBC_MXINT8>(up_scale[i]));
+    const float2 one = make_float2(1.f, 1.f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 s = sigmoid2<DT>(g[k]);
+      const float2 rest = __fadd2_rn(one, make_float2(-s.x, -s.y));
+      dg[k] = __fmul2_rn(__fmul2_rn(dh[k], u[k]), __fmul2_rn(s, __ffma2_rn(g[k], rest, one)));
+      du[k] = __fmul2_rn(dh[k], __fmul2_rn(g[k], s));
+    }
+    store8<DT, VEC>(dgate_at + 16 * i * a.h_stride, dg, cols);
+    store8<DT, VEC>(dup_at + 16 * i * a.dup_stride, du, cols);
   }
 }
 
@@ -118,15 +156,15 @@ bool aligned(const void *p, int64_t stride, int width) {
 }
 
 bool shape(GateArgs &a, int64_t rows, int64_t cols, unsigned *grid) {
-  if (rows <= 0 || cols <= 0 || blocks_of(cols) > INT32_MAX / 4)
+  if (rows <= 0 || cols <= 0)
     return false;
   a.rows = rows;
   a.cols = cols;
-  a.row_units = static_cast<uint32_t>(blocks_of(cols) * 4);
-  a.units = rows * a.row_units;
-  const int64_t n = (a.units + kThreads * kUnits - 1) / (kThreads * kUnits);
+  a.blocks = blocks_of(cols);
+  const int64_t tc = (cols + kTile - 1) / kTile, n = (rows + 16 * kUnits - 1) / (16 * kUnits) * tc;
   if (n > INT32_MAX)
     return false;
+  a.tiles_c = static_cast<uint32_t>(tc);
   *grid = static_cast<unsigned>(n);
   return true;
 }

@@ -18,63 +18,100 @@ struct QuantizeArgs {
   int64_t rows, cols, row_stride;
   uint8_t *codes, *scales;     // blocks along the columns, or NULL
   uint8_t *codes_t, *scales_t; // blocks along the rows: the codes of x^T, or NULL
-  uint32_t *clear;             // words set to zero, or NULL
-  int64_t clear_words;
   uint32_t tiles_c;
 };
 
-/// Blocks along the columns. Thread unit: 8 values of one row; four lanes
-/// share a block (two shuffles for its largest magnitude), sixteen a scale
-/// word. `u` counts the tile's units, 16 per row.
-template <int FMT>
-__device__ __forceinline__ void row_unit(const QuantizeArgs &a, const float (&v)[8], int64_t r, int64_t c) {
-  float m = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    m = abs_max(m, v[i]);
-  m = abs_max(m, __shfl_xor_sync(~0u, m, 1));
-  m = abs_max(m, __shfl_xor_sync(~0u, m, 2));
-  const uint32_t byte = scale_byte<FMT>(m);
+/// Blocks along the columns: a thread holds V = 8 or 16 values of a row, 32 / V
+/// lanes a block (a shuffle each for its largest magnitude). codes and scales
+/// point at this thread's place in the row; `exists`: its block does.
+template <int DT, int FMT, int V>
+__device__ __forceinline__ void row_unit(const Raw8<DT> (&in)[V / 8], uint8_t *codes, uint8_t *scales, bool exists,
+                                         bool row_exists) {
+  float top = in[0].top();
+  if (V == 16)
+    top = fmaxf_bits(top, in[V / 8 - 1].top());
+  const uint32_t byte = scale_byte<FMT>(top_of_lanes<V == 8 ? 2 : 1>(top));
   const float inv = inverse_scale<FMT>(byte);
-  float s[8];
+  uint32_t w[FMT == SBC_MXFP4 ? V / 8 : V / 4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    s[i] = v[i] * inv;
-  const int64_t blocks = blocks_of(a.cols);
-  const bool in = r < a.rows && c < blocks * kBlock;
-  const int lane = threadIdx.x & 31;
-  if (FMT == SBC_MXFP4) {
-    const uint32_t w = byte == 255 ? 0 : codes4(s);
-    if (in)
-      *reinterpret_cast<uint32_t *>(a.codes + r * blocks * 16 + c / 2) = w;
-    // the word of the tile's four blocks; those past the row's end are 0
-    uint32_t word = (c < blocks * kBlock ? byte : 0) << ((lane >> 2 & 3) * 8);
-    word |= __shfl_xor_sync(~0u, word, 4);
-    word |= __shfl_xor_sync(~0u, word, 8);
-    if ((lane & 15) == 0 && r < a.rows)
-      *reinterpret_cast<uint32_t *>(a.scales + scale_word(r, c >> 7, quads_of(a.cols))) = word;
-  } else {
-    uint2 w = make_uint2(codes8x4(s[0], s[1], s[2], s[3]), codes8x4(s[4], s[5], s[6], s[7]));
-    if (byte == 255)
-      w = make_uint2(0, 0);
-    if (in) {
-      *reinterpret_cast<uint2 *>(a.codes + r * blocks * 32 + c) = w;
-      if ((lane & 3) == 0)
-        a.scales[r * blocks + c / 32] = static_cast<uint8_t>(byte);
+  for (int i = 0; i < V / 8; ++i) {
+    float2 v[4];
+    in[i].values(v);
+    if (FMT == SBC_MXFP4) {
+      times(v, inv);
+      w[i] = codes4(v);
+    } else {
+      const uint2 c = codes8(v, inv);
+      w[2 * i] = c.x;
+      w[2 * i + 1] = c.y;
     }
   }
+  constexpr int kWords = sizeof w / 4;
+#pragma unroll
+  for (int i = 0; i < kWords; ++i)
+    if (byte == 255)
+      w[i] = 0;
+  if (exists) {
+    if constexpr (kWords == 1)
+      *reinterpret_cast<uint32_t *>(codes) = w[0];
+    else if constexpr (kWords == 2)
+      *reinterpret_cast<uint2 *>(codes) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint4 *>(codes) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // mxfp4: the bytes of a scale tile's blocks past the row's end are 0
+  if ((threadIdx.x & (32 / V - 1)) == 0 && (FMT == SBC_MXFP4 ? row_exists : exists))
+    *scales = static_cast<uint8_t>(exists ? byte : 0);
 }
 
-template <int DT, int FMT, bool ROWS, bool ACROSS, bool VEC>
+/// Blocks along the columns only: 64 rows (FEW: as many as one unit a thread
+/// covers) x 128 columns per block of threads, the loads of all units before
+/// the first use. 16-bit values go 16 to a thread, which halves the work
+/// per block and per row beside the values' own; with 16 32-bit values the
+/// lanes of a load would lie 64 bytes apart.
+template <int DT, int FMT, bool FEW, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_mx_quantize(const __grid_constant__ QuantizeArgs a) {
   using T = typename Value<DT>::T;
+  constexpr int V = DT == SBC_F32 ? 8 : 16, kLanes = kTile / V, kStride = kThreads / kLanes; // rows between units
+  constexpr int kUnits = FEW ? 1 : 64 / kStride;
   // A kernel launched to overlap this one's end may begin its own set-up; it
   // waits for this grid's completion before it reads what is written here.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x - tr * a.tiles_c;
+  const int row = threadIdx.x / kLanes, c8 = threadIdx.x % kLanes * V;
+  const int64_t r0 = static_cast<int64_t>(tr) * (kUnits * kStride) + row;
+  const int64_t c = static_cast<int64_t>(tc) * kTile + c8, left = a.cols - c;
+  const int have = static_cast<int>(left < 0 ? 0 : left < V ? left : V);
+  const T *x = static_cast<const T *>(a.x) + r0 * a.row_stride + c;
+  const int rows = static_cast<int>(a.rows - r0 < 64 ? a.rows - r0 : 64); // from r0 on
+  Raw8<DT> in[kUnits][V / 8];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i)
+#pragma unroll
+    for (int j = 0; j < V / 8; ++j)
+      in[i][j].template load<VEC>(x + i * kStride * a.row_stride + 8 * j, i * kStride < rows ? have - 8 * j : 0);
+  const int64_t blocks = blocks_of(a.cols);
+  const bool exists = c < blocks * kBlock;
+  constexpr int kBytes = FMT == SBC_MXFP4 ? 16 : 32; // of codes per block
+  uint8_t *codes = a.codes + r0 * blocks * kBytes + c * kBytes / 32;
+  const int64_t code_step = blocks * (kBytes * kStride);
+  uint8_t *scales = a.scales + (FMT == SBC_MXFP4 ? scale_word(r0, tc, quads_of(a.cols)) + c8 / 32 : r0 * blocks + c / 32);
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    // mxfp4, 64 rows from a multiple of 64: within a scale tile 32 rows are 4
+    // bytes and one row 16
+    const int64_t scale_step = FMT == SBC_MXFP4 ? (i * kStride / 32) * 4 + (i * kStride % 32) * 16 : i * kStride * blocks;
+    const bool row_exists = i * kStride < rows;
+    row_unit<DT, FMT, V>(in[i], codes + i * code_step, scales + scale_step, row_exists && exists, row_exists);
+  }
+}
+
+/// Blocks along the rows, and with ROWS along the columns too, from one read:
+/// a tile of 128 x 128 values.
+template <int DT, bool ROWS, bool VEC>
+__global__ void __launch_bounds__(kThreads) k_mx_quantize_across(const __grid_constant__ QuantizeArgs a) {
+  using T = typename Value<DT>::T;
   const int t = threadIdx.x;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + t; i < a.clear_words;
-       i += static_cast<int64_t>(gridDim.x) * kThreads)
-    a.clear[i] = 0;
   const uint32_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x - tr * a.tiles_c;
   const int64_t r0 = static_cast<int64_t>(tr) * kTile, c0 = static_cast<int64_t>(tc) * kTile;
   const T *x = static_cast<const T *>(a.x);
@@ -82,80 +119,85 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize(const __grid_constant_
   const int64_t c = c0 + c8;
   const int have = static_cast<int>(a.cols - c < 0 ? 0 : a.cols - c < 8 ? a.cols - c : 8);
   const int here = static_cast<int>(a.rows - r0 < kTile ? a.rows - r0 : kTile);
-
-  if constexpr (!ACROSS) {
-#pragma unroll 4
-    for (int i = 0; i < 8; ++i) {
-      const int row = (t >> 4) + 16 * i;
-      if ((row & ~1) >= here) // the warp's two rows
-        break;
-      float v[8];
-      load8<DT, VEC>(v, x + (r0 + row) * a.row_stride + c, row < here ? have : 0);
-      row_unit<FMT>(a, v, r0 + row, c);
+  extern __shared__ uint4 smem[];
+  T *tile = reinterpret_cast<T *>(smem);                           // [128][128]
+  uint4 *codes = smem + kTile * kTile * sizeof(T) / 16;            // [128 columns][4]
+  uint8_t *scales = reinterpret_cast<uint8_t *>(codes + kTile * 4); // [512]
+  const int64_t row_blocks = blocks_of(a.cols);
+  uint8_t *row_codes = a.codes + (r0 + (t >> 4)) * row_blocks * 16 + c / 2;
+  uint8_t *row_scales = a.scales + scale_word(r0 + (t >> 4), tc, quads_of(a.cols)) + c8 / 32;
+  Raw8<DT> in[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = (t >> 4) + 16 * i;
+    in[i].template load<VEC>(x + (r0 + row) * a.row_stride + c, row < here ? have : 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = (t >> 4) + 16 * i;
+    *reinterpret_cast<Raw8<DT> *>(tile + row * kTile + c8) = in[i];
+    if (ROWS && (row & ~1) < here) // the warp's two rows
+      row_unit<DT, SBC_MXFP4, 8>(*reinterpret_cast<const Raw8<DT>(*)[1]>(&in[i]), row_codes + i * (16 * row_blocks * 16),
+                                 row_scales + (i / 2) * 4 + (i % 2) * 256, row < here && c < row_blocks * kBlock,
+                                 row < here);
+  }
+  __syncthreads();
+  // Blocks along the rows: a thread takes 32 rows of two neighbouring 16-bit
+  // columns, or of two 32-bit columns 64 apart, so that the lanes of a warp
+  // read neighbouring words and no bank is hit twice.
+  const int rb = t >> 6, word = t & 63;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    if (DT != SBC_F32 && half)
+      break;
+    constexpr int kCols = DT == SBC_F32 ? 1 : 2;
+    const int col = DT == SBC_F32 ? word + 64 * half : 2 * word;
+    uint32_t w[32], m = 0; // m: the largest magnitudes, as bits
+#pragma unroll
+    for (int k = 0; k < 32; ++k) {
+      w[k] = *reinterpret_cast<const uint32_t *>(tile + (rb * 32 + k) * kTile + col);
+      m = DT == SBC_F32 ? max(m, w[k] & 0x7fffffffu) : __vmaxu2(m, w[k] & 0x7fff7fffu);
     }
-  } else {
-    extern __shared__ uint4 smem[];
-    T *tile = reinterpret_cast<T *>(smem);                           // [128][128]
-    uint4 *codes = smem + kTile * kTile * sizeof(T) / 16;            // [128 columns][4]
-    uint8_t *scales = reinterpret_cast<uint8_t *>(codes + kTile * 4); // [512]
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = (t >> 4) + 16 * i;
-      float v[8];
-      load8<DT, VEC>(v, x + (r0 + row) * a.row_stride + c, row < here ? have : 0);
-      T *d = tile + row * kTile + c8;
-      T raw[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        raw[k] = Value<DT>::down(v[k]);
-#pragma unroll
-      for (int k = 0; k < static_cast<int>(sizeof raw / 16); ++k)
-        reinterpret_cast<uint4 *>(d)[k] = reinterpret_cast<const uint4 *>(raw)[k];
-      if (ROWS && (row & ~1) < here)
-        row_unit<FMT>(a, v, r0 + row, c);
-    }
-    __syncthreads();
-    // Blocks along the rows: a thread takes 32 rows of one column. The lanes
-    // of a warp read neighbouring columns, so no bank is hit twice.
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int col = t & 127, rb = (t >> 7) + 2 * i;
-      float v[32];
-      float m = 0.f;
-#pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        v[k] = Value<DT>::up(tile[(rb * 32 + k) * kTile + col]);
-        m = abs_max(m, v[k]);
-      }
-      const uint32_t byte = scale_byte<SBC_MXFP4>(m);
+    for (int j = 0; j < kCols; ++j) {
+      float2 top = make_float2(__uint_as_float(m), 0.f);
+      if (DT != SBC_F32)
+        top = unpack2<DT>(m);
+      const uint32_t byte = scale_byte<SBC_MXFP4>(j ? top.y : top.x);
       const float inv = inverse_scale<SBC_MXFP4>(byte);
-      uint32_t w[4];
+      uint32_t out[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float s[8];
+        float2 s[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          s[j] = v[8 * k + j] * inv;
-        w[k] = byte == 255 ? 0 : codes4(s);
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x0 = w[8 * k + 2 * i], x1 = w[8 * k + 2 * i + 1];
+          if (DT == SBC_F32)
+            s[i] = make_float2(__uint_as_float(x0), __uint_as_float(x1));
+          else // column j of both rows
+            s[i] = unpack2<DT>(__byte_perm(x0, x1, j ? 0x7632 : 0x5410));
+        }
+        times(s, inv);
+        out[k] = byte == 255 ? 0 : codes4(s);
       }
-      codes[col * 4 + (rb ^ (col >> 1 & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
-      scales[(col & 31) * 16 + (col >> 5) * 4 + rb] = static_cast<uint8_t>(r0 + rb * 32 < a.rows ? byte : 0);
+      codes[(col + j) * 4 + (rb ^ (col >> 1 & 3))] = make_uint4(out[0], out[1], out[2], out[3]);
+      scales[(col + j & 31) * 16 + (col + j >> 5) * 4 + rb] = static_cast<uint8_t>(r0 + rb * 32 < a.rows ? byte : 0);
     }
-    __syncthreads();
-    const int64_t blocks = blocks_of(a.rows), quads = quads_of(a.rows);
+  }
+  __syncthreads();
+  const int64_t blocks = blocks_of(a.rows), quads = quads_of(a.rows);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int col = (t >> 2) + 64 * i, rb = t & 3;
-      if (c0 + col < a.cols && r0 / 32 + rb < blocks)
-        *reinterpret_cast<uint4 *>(a.codes_t + (c0 + col) * blocks * 16 + (r0 / 32 + rb) * 16) =
-            codes[col * 4 + (rb ^ (col >> 1 & 3))];
-    }
-    if (t < 128) { // rows of the scale tile past the last column stay as they were
-      const int col = (t >> 2) + 32 * (t & 3);
-      if (c0 + col < a.cols)
-        *reinterpret_cast<uint32_t *>(a.scales_t + scale_word(c0 + col, tr, quads)) =
-            reinterpret_cast<const uint32_t *>(scales)[t];
-    }
+  for (int i = 0; i < 2; ++i) {
+    const int col = (t >> 2) + 64 * i, rb = t & 3;
+    if (c0 + col < a.cols && r0 / 32 + rb < blocks)
+      *reinterpret_cast<uint4 *>(a.codes_t + (c0 + col) * blocks * 16 + (r0 / 32 + rb) * 16) =
+          codes[col * 4 + (rb ^ (col >> 1 & 3))];
+  }
+  if (t < 128) { // rows of the scale tile past the last column stay as they were
+    const int col = (t >> 2) + 32 * (t & 3);
+    if (c0 + col < a.cols)
+      *reinterpret_cast<uint32_t *>(a.scales_t + scale_word(c0 + col, tr, quads)) =
+          reinterpret_cast<const uint32_t *>(scales)[t];
   }
 }
 
@@ -163,41 +205,71 @@ struct DequantizeArgs {
   const uint8_t *codes, *scales;
   void *out;
   int64_t rows, cols;
-  uint32_t tiles_c;
+  uint32_t tiles_c, tiles;
 };
 
-/// Codes to values, in the layout of the codes: [rows, cols]. Thread unit as
-/// in k_mx_quantize.
-template <int DT, int FMT, bool VEC>
+/// Codes to values, in the layout of the codes: [rows, cols]. A thread takes 8
+/// values of a row (4 of 32 bits, so that a warp's stores are contiguous) in
+/// each of its units, whose loads all come first.
+template <int DT, int FMT, bool FEW, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const __grid_constant__ DequantizeArgs a) {
   using T = typename Value<DT>::T;
+  constexpr int V = DT == SBC_F32 ? 4 : 8, kLanes = kTile / V, kStride = kThreads / kLanes;
+  constexpr int kUnits = FEW ? 1 : 64 / kStride;
+  constexpr int kBytes = FMT == SBC_MXFP4 ? 16 : 32; // of codes per block
+  using C = typename std::conditional<V * kBytes / 32 == 8, uint2, uint32_t>::type;
   const uint32_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x - tr * a.tiles_c;
-  const int64_t r0 = static_cast<int64_t>(tr) * kTile;
-  const int t = threadIdx.x;
-  const int64_t c = static_cast<int64_t>(tc) * kTile + (t & 15) * 8;
-  const int have = static_cast<int>(a.cols - c < 8 ? a.cols - c : 8);
-  const int64_t blocks = blocks_of(a.cols), quads = quads_of(a.cols);
-  if (have <= 0)
+  const int c8 = threadIdx.x % kLanes * V;
+  const int64_t r0 = static_cast<int64_t>(tr) * (kUnits * kStride) + threadIdx.x / kLanes;
+  const int64_t c = static_cast<int64_t>(tc) * kTile + c8, left = a.cols - c;
+  const int have = static_cast<int>(left < V ? left : V);
+  const int rows = static_cast<int>(a.rows - r0 < 64 ? a.rows - r0 : 64); // from r0 on
+  if (have <= 0 || rows <= 0)
     return;
-#pragma unroll 4
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + (t >> 4) + 16 * i;
-    if (r >= a.rows)
-      return;
-    float v[8], s;
-    if (FMT == SBC_MXFP4) {
-      values4(v, __ldg(reinterpret_cast<const uint32_t *>(a.codes + r * blocks * 16 + c / 2)));
-      s = scale_value<FMT>(__ldg(a.scales + scale_word(r, c >> 7, quads) + (c >> 5 & 3)));
-    } else {
-      const uint2 w = __ldg(reinterpret_cast<const uint2 *>(a.codes + r * blocks * 32 + c));
-      values8x4(v, w.x);
-      values8x4(v + 4, w.y);
-      s = scale_value<FMT>(__ldg(a.scales + r * blocks + c / 32));
-    }
+  const int64_t blocks = blocks_of(a.cols);
+  // four 4-bit codes are half a word, which two lanes read
+  const uint8_t *codes_at = a.codes + r0 * blocks * kBytes + (c * kBytes / 32 & ~int64_t{3});
+  const int shift = V * kBytes / 32 == 2 ? static_cast<int>(c & 4) * 4 : 0;
+  const uint8_t *scales = a.scales + (FMT == SBC_MXFP4 ? scale_word(r0, tc, quads_of(a.cols)) + c8 / 32 : r0 * blocks + c / 32);
+  C codes[kUnits];
+  uint32_t scale[kUnits];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      v[k] *= s;
-    store8<DT, VEC>(static_cast<T *>(a.out) + r * a.cols + c, v, have);
+  for (int i = 0; i < kUnits; ++i)
+    if (i * kStride < rows) {
+      const int64_t step = FMT == SBC_MXFP4 ? (i * kStride / 32) * 4 + (i * kStride % 32) * 16 : i * kStride * blocks;
+      codes[i] = __ldg(reinterpret_cast<const C *>(codes_at + i * (kStride * kBytes) * blocks));
+      scale[i] = __ldg(scales + step);
+    }
+  T *out = static_cast<T *>(a.out) + r0 * a.cols + c;
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    if (i * kStride >= rows)
+      return;
+    float2 v[4];
+    const float s = scale_value<FMT>(scale[i]);
+    if constexpr (FMT == SBC_MXFP4) {
+      values4(v, codes[i] >> shift);
+      times(v, s);
+    } else {
+      uint2 w = make_uint2(0, 0);
+      if constexpr (V == 8)
+        w = codes[i];
+      else
+        w.x = codes[i];
+      values8(v, w, s);
+    }
+    T *p = out + i * kStride * a.cols;
+    if constexpr (V == 8) {
+      store8<DT, VEC>(p, v, have);
+    } else if (VEC && have >= 4) {
+      __stcs(reinterpret_cast<float4 *>(p), make_float4(v[0].x, v[0].y, v[1].x, v[1].y));
+    } else {
+      const float e[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < have)
+          p[k] = Value<DT>::down(e[k]);
+    }
   }
 }
 
@@ -206,62 +278,78 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const __grid_constan
 /// reads one word (8 columns) of each of 8 consecutive rows, the lanes of a
 /// warp 16 row groups x 2 words on 32 distinct banks, and writes 8 values of
 /// each column as one run (128 values of a column per half-warp).
+/// A block takes every gridDim-th tile; the next tile's codes and scales are
+/// on their way to registers while this one's values are stored.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_mx_dequantize_t(const __grid_constant__ DequantizeArgs a) {
   using T = typename Value<DT>::T;
   constexpr int kPitch = 18;
-  __shared__ uint32_t codes[kTile * kPitch];
-  __shared__ uint32_t scales[kTile];
-  const uint32_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x - tr * a.tiles_c;
-  const int64_t r0 = static_cast<int64_t>(tr) * kTile, c0 = static_cast<int64_t>(tc) * kTile;
+  __shared__ uint32_t codes[2][kTile * kPitch];
+  __shared__ uint32_t scales[2][kTile];
   const int64_t blocks = blocks_of(a.cols), quads = quads_of(a.cols);
   const int t = threadIdx.x;
+  uint4 next[2];
+  uint32_t next_scale = 0;
+  const auto fetch = [&](uint32_t tile) {
+    const uint32_t tr = tile / a.tiles_c, tc = tile - tr * a.tiles_c;
+    const int64_t r0 = static_cast<int64_t>(tr) * kTile, block = static_cast<int64_t>(tc) * 4 + (t & 3);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = (t >> 2) + 64 * i, q = t & 3;
-    if (r0 + row < a.rows && c0 / 32 + q < blocks) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4 *>(a.codes + (r0 + row) * blocks * 16 + (c0 / 32 + q) * 16));
-      uint32_t *d = codes + (16 * (row & 7) + row / 8) * kPitch + 4 * q;
-      reinterpret_cast<uint2 *>(d)[0] = make_uint2(w.x, w.y);
-      reinterpret_cast<uint2 *>(d)[1] = make_uint2(w.z, w.w);
+    for (int i = 0; i < 2; ++i) {
+      const int64_t r = r0 + (t >> 2) + 64 * i;
+      if (r < a.rows && block < blocks)
+        next[i] = __ldg(reinterpret_cast<const uint4 *>(a.codes + (r * blocks + block) * 16));
     }
-  }
-  if (t < kTile && r0 + t < a.rows)
-    scales[t] = __ldg(reinterpret_cast<const uint32_t *>(a.scales + scale_word(r0 + t, tc, quads)));
-  __syncthreads();
-  const int ag = t & 15, c = t >> 4; // rows 8 ag + i, columns 8 c + j
-  const int64_t r = r0 + 8 * ag;
-  const int have = static_cast<int>(a.rows - r < 8 ? a.rows - r : 8);
-  if (have <= 0 || c0 + 8 * c >= a.cols)
-    return;
-  float v[8][8];
+    if (t < kTile && r0 + t < a.rows)
+      next_scale = __ldg(reinterpret_cast<const uint32_t *>(a.scales + scale_word(r0 + t, tc, quads)));
+  };
+  if (blockIdx.x < a.tiles)
+    fetch(blockIdx.x);
+  int buf = 0;
+  for (uint32_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, buf ^= 1) {
+    const uint32_t tr = tile / a.tiles_c, tc = tile - tr * a.tiles_c;
+    const int64_t r0 = static_cast<int64_t>(tr) * kTile, c0 = static_cast<int64_t>(tc) * kTile;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (i >= have) { // rows past the end: nothing was staged
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[i][j] = 0.f;
+    for (int i = 0; i < 2; ++i) {
+      const int row = (t >> 2) + 64 * i;
+      uint2 *d = reinterpret_cast<uint2 *>(codes[buf] + (16 * (row & 7) + row / 8) * kPitch + 4 * (t & 3));
+      d[0] = make_uint2(next[i].x, next[i].y);
+      d[1] = make_uint2(next[i].z, next[i].w);
+    }
+    if (t < kTile)
+      scales[buf][t] = next_scale;
+    __syncthreads(); // the other buffer's readers are past it: they wrote this one before
+    if (tile + gridDim.x < a.tiles)
+      fetch(tile + gridDim.x);
+    const int ag = t & 15, c = t >> 4; // rows 8 ag + i, columns 8 c + j
+    const int64_t r = r0 + 8 * ag;
+    const int have = static_cast<int>(a.rows - r < 8 ? a.rows - r : 8);
+    if (have <= 0 || c0 + 8 * c >= a.cols)
       continue;
+    // what was staged for rows past the end is never stored
+    float2 v[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      values4(v[i], codes[buf][(16 * i + ag) * kPitch + c]);
+      times(v[i], scale_value<SBC_MXFP4>(scales[buf][8 * ag + i] >> (c >> 2) * 8 & 255));
     }
-    values4(v[i], codes[(16 * i + ag) * kPitch + c]);
-    const float s = scale_value<SBC_MXFP4>(scales[8 * ag + i] >> (c >> 2) * 8 & 255);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      v[i][j] *= s;
-  }
+    for (int j = 0; j < 8; ++j) {
+      if (c0 + 8 * c + j >= a.cols)
+        break;
+      float2 col[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (c0 + 8 * c + j >= a.cols)
-      return;
-    const float col[8] = {v[0][j], v[1][j], v[2][j], v[3][j], v[4][j], v[5][j], v[6][j], v[7][j]};
-    store8<DT, VEC>(static_cast<T *>(a.out) + (c0 + 8 * c + j) * a.rows + r, col, have);
+      for (int i = 0; i < 4; ++i)
+        col[i] = j & 1 ? make_float2(v[2 * i][j / 2].y, v[2 * i + 1][j / 2].y)
+                       : make_float2(v[2 * i][j / 2].x, v[2 * i + 1][j / 2].x);
+      store8<DT, VEC>(static_cast<T *>(a.out) + (c0 + 8 * c + j) * a.rows + r, col, have);
+    }
   }
 }
 
 int width(int dt) { return dt == SBC_F32 ? 4 : 2; }
 
-bool grid_of(int64_t rows, int64_t cols, uint32_t *tiles_c, uint32_t *grid) {
-  const int64_t tc = (cols + kTile - 1) / kTile, n = ((rows + kTile - 1) / kTile) * tc;
+bool grid_of(int64_t rows, int64_t cols, int tile_rows, uint32_t *tiles_c, uint32_t *grid) {
+  const int64_t tc = (cols + kTile - 1) / kTile, n = ((rows + tile_rows - 1) / tile_rows) * tc;
   if (n > INT32_MAX)
     return false;
   *tiles_c = static_cast<uint32_t>(tc);
@@ -269,15 +357,14 @@ bool grid_of(int64_t rows, int64_t cols, uint32_t *tiles_c, uint32_t *grid) {
   return true;
 }
 
-template <int DT, bool VEC> int launch_quantize(const QuantizeArgs &a, int fmt, uint32_t grid, cudaStream_t s) {
+template <int DT, bool VEC> int launch_quantize(const QuantizeArgs &a, int fmt, bool few, uint32_t grid, cudaStream_t s) {
   if (!a.codes_t) {
-    if (fmt == SBC_MXFP4)
-      k_mx_quantize<DT, SBC_MXFP4, true, false, VEC><<<grid, kThreads, 0, s>>>(a);
-    else
-      k_mx_quantize<DT, SBC_MXINT8, true, false, VEC><<<grid, kThreads, 0, s>>>(a);
+    auto k = few ? (fmt == SBC_MXFP4 ? k_mx_quantize<DT, SBC_MXFP4, true, VEC> : k_mx_quantize<DT, SBC_MXINT8, true, VEC>)
+                 : (fmt == SBC_MXFP4 ? k_mx_quantize<DT, SBC_MXFP4, false, VEC> : k_mx_quantize<DT, SBC_MXINT8, false, VEC>);
+    k<<<grid, kThreads, 0, s>>>(a);
   } else {
     const int bytes = kTile * kTile * static_cast<int>(sizeof(typename Value<DT>::T)) + kTile * 64 + 512;
-    auto k = a.codes ? k_mx_quantize<DT, SBC_MXFP4, true, true, VEC> : k_mx_quantize<DT, SBC_MXFP4, false, true, VEC>;
+    auto k = a.codes ? k_mx_quantize_across<DT, true, VEC> : k_mx_quantize_across<DT, false, VEC>;
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess)
       return e;
@@ -288,28 +375,36 @@ template <int DT, bool VEC> int launch_quantize(const QuantizeArgs &a, int fmt, 
 }
 
 template <int DT, bool VEC>
-int launch_dequantize(const DequantizeArgs &a, int fmt, int transpose, uint32_t grid, cudaStream_t s) {
-  if (transpose)
+int launch_dequantize(const DequantizeArgs &a, int fmt, int transpose, bool few, uint32_t grid, cudaStream_t s) {
+  if (transpose) {
     k_mx_dequantize_t<DT, VEC><<<grid, kThreads, 0, s>>>(a);
-  else if (fmt == SBC_MXFP4)
-    k_mx_dequantize<DT, SBC_MXFP4, VEC><<<grid, kThreads, 0, s>>>(a);
-  else
-    k_mx_dequantize<DT, SBC_MXINT8, VEC><<<grid, kThreads, 0, s>>>(a);
+  } else {
+    auto k =
+        few ? (fmt == SBC_MXFP4 ? k_mx_dequantize<DT, SBC_MXFP4, true, VEC> : k_mx_dequantize<DT, SBC_MXINT8, true, VEC>)
+            : (fmt == SBC_MXFP4 ? k_mx_dequantize<DT, SBC_MXFP4, false, VEC> : k_mx_dequantize<DT, SBC_MXINT8, false, VEC>);
+    k<<<grid, kThreads, 0, s>>>(a);
+  }
   sbc::count_launch();
   return cudaGetLastError();
 }
+
+/// Whether the row-by-row kernels take one unit a thread: while that fills the
+/// SMs at most twice over, a few tokens wait for one load's latency (and more
+/// blocks share it) instead of four loads' issue.
+bool few_of(int64_t rows, int64_t cols) { return rows * ((cols + kTile - 1) / kTile) <= 16 * 2048; }
 
 } // namespace
 
 extern "C" {
 
 int sbc_mx_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols, int64_t row_stride, const sbc_mx *along,
-                    const sbc_mx *across, uint32_t *clear, int64_t clear_words, void *stream) {
+                    const sbc_mx *across, void *stream) {
   QuantizeArgs a{};
   uint32_t grid = 0;
+  const bool few = few_of(rows, cols);
   if (!x || rows <= 0 || cols <= 0 || (!along && !across) || (across && across->format != SBC_MXFP4) ||
       (along && across && along->format != SBC_MXFP4) || dtype < SBC_F32 || dtype > SBC_BF16 ||
-      !grid_of(rows, cols, &a.tiles_c, &grid))
+      !grid_of(rows, cols, across ? kTile : few ? (dtype == SBC_F32 ? 16 : 32) : 64, &a.tiles_c, &grid))
     return SBC_EINVAL;
   a.x = x;
   a.rows = rows;
@@ -319,27 +414,29 @@ int sbc_mx_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols, in
   a.scales = along ? static_cast<uint8_t *>(along->scales) : nullptr;
   a.codes_t = across ? static_cast<uint8_t *>(across->codes) : nullptr;
   a.scales_t = across ? static_cast<uint8_t *>(across->scales) : nullptr;
-  a.clear = clear;
-  a.clear_words = clear ? clear_words : 0;
   const int fmt = along ? along->format : static_cast<int>(SBC_MXFP4);
   const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && row_stride * width(dtype) % 16 == 0;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
   case SBC_F32:
-    return vec ? launch_quantize<SBC_F32, true>(a, fmt, grid, s) : launch_quantize<SBC_F32, false>(a, fmt, grid, s);
+    return vec ? launch_quantize<SBC_F32, true>(a, fmt, few, grid, s) : launch_quantize<SBC_F32, false>(a, fmt, few, grid, s);
   case SBC_F16:
-    return vec ? launch_quantize<SBC_F16, true>(a, fmt, grid, s) : launch_quantize<SBC_F16, false>(a, fmt, grid, s);
+    return vec ? launch_quantize<SBC_F16, true>(a, fmt, few, grid, s) : launch_quantize<SBC_F16, false>(a, fmt, few, grid, s);
   default:
-    return vec ? launch_quantize<SBC_BF16, true>(a, fmt, grid, s) : launch_quantize<SBC_BF16, false>(a, fmt, grid, s);
+    return vec ? launch_quantize<SBC_BF16, true>(a, fmt, few, grid, s) : launch_quantize<SBC_BF16, false>(a, fmt, few, grid, s);
   }
 }
 
 int sbc_mx_dequantize(const sbc_mx *q, void *out, int32_t dtype, int32_t transpose, void *stream) {
   DequantizeArgs a{};
   uint32_t grid = 0;
+  const bool few = q && few_of(q->rows, q->cols);
   if (!q || !out || q->rows <= 0 || q->cols <= 0 || (transpose && q->format != SBC_MXFP4) || dtype < SBC_F32 ||
-      dtype > SBC_BF16 || !grid_of(q->rows, q->cols, &a.tiles_c, &grid))
+      dtype > SBC_BF16 || !grid_of(q->rows, q->cols, transpose ? kTile : few ? (dtype == SBC_F32 ? 8 : 16) : 64, &a.tiles_c, &grid))
     return SBC_EINVAL;
+  a.tiles = grid;
+  if (transpose && grid > 148 * 3) // three blocks stay on each SM
+    grid = 148 * 3;
   a.codes = static_cast<const uint8_t *>(q->codes);
   a.scales = static_cast<const uint8_t *>(q->scales);
   a.out = out;
@@ -350,14 +447,14 @@ int sbc_mx_dequantize(const sbc_mx *q, void *out, int32_t dtype, int32_t transpo
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
   case SBC_F32:
-    return vec ? launch_dequantize<SBC_F32, true>(a, q->format, transpose, grid, s)
-               : launch_dequantize<SBC_F32, false>(a, q->format, transpose, grid, s);
+    return vec ? launch_dequantize<SBC_F32, true>(a, q->format, transpose, few, grid, s)
+               : launch_dequantize<SBC_F32, false>(a, q->format, transpose, few, grid, s);
   case SBC_F16:
-    return vec ? launch_dequantize<SBC_F16, true>(a, q->format, transpose, grid, s)
-               : launch_dequantize<SBC_F16, false>(a, q->format, transpose, grid, s);
+    return vec ? launch_dequantize<SBC_F16, true>(a, q->format, transpose, few, grid, s)
+               : launch_dequantize<SBC_F16, false>(a, q->format, transpose, few, grid, s);
   default:
-    return vec ? launch_dequantize<SBC_BF16, true>(a, q->format, transpose, grid, s)
-               : launch_dequantize<SBC_BF16, false>(a, q->format, transpose, grid, s);
+    return vec ? launch_dequantize<SBC_BF16, true>(a, q->format, transpose, few, grid, s)
+               : launch_dequantize<SBC_BF16, false>(a, q->format, transpose, few, grid, s);
   }
 }
 

@@ -27,6 +27,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace mx {
 
@@ -58,54 +59,127 @@ template <> struct Value<SBC_BF16> {
   static __device__ __forceinline__ T down(float v) { return __float2bfloat16_rn(v); }
 };
 
-/// Eight consecutive values at p; `have` of them exist (the rest read as
-/// zero). VEC: p is 16-byte aligned.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load8(float (&v)[8], const typename Value<DT>::T *p, int have) {
-  using T = typename Value<DT>::T;
-  if (VEC && have >= 8) {
-    T raw[8];
-    const uint4 *s = reinterpret_cast<const uint4 *>(p);
-    uint4 *d = reinterpret_cast<uint4 *>(raw);
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof raw / 16); ++i)
-      d[i] = __ldg(s + i);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = Value<DT>::up(raw[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = i < have ? Value<DT>::up(p[i]) : 0.f;
-  }
+/// A pair of 16-bit values in 32 bits each.
+template <int DT> __device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if (DT == SBC_F16)
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+/// Two values rounded to 16 bits, the first in the lower half.
+template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  uint32_t r;
+  if (DT == SBC_F16)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
 }
 
+/// Eight consecutive values as they lie in memory. Loading and converting are
+/// apart so that a thread's loads can all be on their way before the first is
+/// waited for.
+template <int DT> struct Raw8 {
+  uint4 q[DT == SBC_F32 ? 2 : 1];
+
+  /// The values at p, of which `have` exist; the rest are zero. VEC: p is
+  /// 16-byte aligned.
+  template <bool VEC> __device__ __forceinline__ void load(const typename Value<DT>::T *p, int have) {
+    if (VEC && have >= 8) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof q / 16); ++i)
+        q[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    } else {
+      using U = typename std::conditional<DT == SBC_F32, uint32_t, uint16_t>::type;
+      const U *u = reinterpret_cast<const U *>(p);
+      U v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = i < have ? __ldg(u + i) : U(0);
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof q / 4); ++i) {
+        uint32_t w;
+        if (DT == SBC_F32)
+          w = v[i];
+        else
+          w = v[2 * i & 7] | static_cast<uint32_t>(v[2 * i + 1 & 7]) << 16;
+        reinterpret_cast<uint32_t *>(q)[i] = w;
+      }
+    }
+  }
+
+  /// The values as four pairs in 32 bits.
+  __device__ __forceinline__ void values(float2 (&v)[4]) const {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (DT == SBC_F32)
+        v[i] = make_float2(__uint_as_float(w[2 * i & 7]), __uint_as_float(w[2 * i + 1 & 7]));
+      else
+        v[i] = unpack2<DT>(w[i]);
+    }
+  }
+
+  /// The largest magnitude, a NaN above all. Magnitudes order like their bits,
+  /// so 16-bit values are compared two at a time as whole numbers.
+  __device__ __forceinline__ float top() const {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(q);
+    if (DT == SBC_F32) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        m = max(m, w[i & 7] & 0x7fffffffu);
+      return __uint_as_float(m);
+    }
+    uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+      m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+    m = max(m & 0xffffu, m >> 16);
+    return unpack2<DT>(m).x;
+  }
+};
+
+/// The larger of two magnitudes, a NaN above all.
+__device__ __forceinline__ float fmaxf_bits(float a, float b) {
+  return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
+}
+
+/// The largest magnitude over the 2^n lanes of a block's quarters; magnitudes
+/// and NaN order like their bits.
+template <int N> __device__ __forceinline__ float top_of_lanes(float m) {
+  uint32_t u = __float_as_uint(m);
+#pragma unroll
+  for (int i = 1; i < 1 << N; i *= 2)
+    u = max(u, __shfl_xor_sync(~0u, u, i));
+  return __uint_as_float(u);
+}
+
+/// Eight values to p, of which `have` exist; VEC: p is 16-byte aligned.
 template <int DT, bool VEC>
-__device__ __forceinline__ void store8(typename Value<DT>::T *p, const float (&v)[8], int have) {
-  using T = typename Value<DT>::T;
+__device__ __forceinline__ void store8(typename Value<DT>::T *p, const float2 (&v)[4], int have) {
+  uint4 q[DT == SBC_F32 ? 2 : 1];
+  uint32_t *w = reinterpret_cast<uint32_t *>(q);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (DT == SBC_F32) {
+      w[2 * i & 7] = __float_as_uint(v[i].x);
+      w[2 * i + 1 & 7] = __float_as_uint(v[i].y);
+    } else {
+      w[i] = pack2<DT>(v[i].x, v[i].y);
+    }
+  }
   if (VEC && have >= 8) {
-    T raw[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      raw[i] = Value<DT>::down(v[i]);
-    const uint4 *s = reinterpret_cast<const uint4 *>(raw);
-    uint4 *d = reinterpret_cast<uint4 *>(p);
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof raw / 16); ++i)
-      __stcs(d + i, s[i]);
+    for (int i = 0; i < static_cast<int>(sizeof q / 16); ++i)
+      __stcs(reinterpret_cast<uint4 *>(p) + i, q[i]);
   } else {
+    using U = typename std::conditional<DT == SBC_F32, uint32_t, uint16_t>::type;
+    U *u = reinterpret_cast<U *>(p);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i < have)
-        p[i] = Value<DT>::down(v[i]);
+        u[i] = DT == SBC_F32 ? static_cast<U>(w[i & 7]) : static_cast<U>(w[i >> 1] >> (i & 1) * 16);
   }
-}
-
-/// max(a, |b|) that keeps a NaN.
-__device__ __forceinline__ float abs_max(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
-  return r;
 }
 
 /// Scale byte of a block whose largest magnitude is amax. The exponent field
@@ -138,28 +212,44 @@ template <int FMT> __device__ __forceinline__ float scale_value(uint32_t byte) {
   return power(FMT == SBC_MXFP4 ? static_cast<int>(byte) : static_cast<int>(byte) - 6);
 }
 
-/// Eight 4-bit codes of v[0..7] (already divided by the scale).
-__device__ __forceinline__ uint32_t codes4(const float (&v)[8]) {
+/// v times one factor.
+__device__ __forceinline__ void times(float2 (&v)[4], float f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] = __fmul2_rn(v[i], make_float2(f, f));
+}
+
+/// Eight 4-bit codes of v (already divided by the scale).
+__device__ __forceinline__ uint32_t codes4(const float2 (&v)[4]) {
   uint32_t r;
   asm("{\n .reg .b8 a, b, c, d;\n"
       " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
       " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
       " mov.b32 %0, {a, b, c, d};\n}"
       : "=r"(r)
-      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+      : "f"(v[0].x), "f"(v[0].y), "f"(v[1].x), "f"(v[1].y), "f"(v[2].x), "f"(v[2].y), "f"(v[3].x), "f"(v[3].y));
   return r;
 }
 
-/// One 8-bit code: rne(v) clamped to +-127.
-__device__ __forceinline__ uint32_t code8(float v) {
-  return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(v, -127.f), 127.f))) & 255u;
-}
-__device__ __forceinline__ uint32_t codes8x4(float a, float b, float c, float d) {
-  return code8(a) | (code8(b) << 8) | (code8(c) << 16) | (code8(d) << 24);
+/// Eight 8-bit codes rne(v inv) clamped to +-127. Adding 1.5 2^23 in the same
+/// step rounds the exact product to a whole number (ties to even) and leaves
+/// its two's complement in the low byte: no conversion instruction, whose unit
+/// the exponentials need.
+__device__ __forceinline__ uint2 codes8(const float2 (&v)[4], float inv) {
+  constexpr float kWhole = 12582912.f;
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __ffma2_rn(v[i], make_float2(inv, inv), make_float2(kWhole, kWhole));
+    w[2 * i] = __float_as_uint(fminf(fmaxf(t.x, kWhole - 127.f), kWhole + 127.f));
+    w[2 * i + 1] = __float_as_uint(fminf(fmaxf(t.y, kWhole - 127.f), kWhole + 127.f));
+  }
+  return make_uint2(__byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410));
 }
 
 /// The values (before the scale) of eight 4-bit codes.
-__device__ __forceinline__ void values4(float (&v)[8], uint32_t codes) {
+__device__ __forceinline__ void values4(float2 (&v)[4], uint32_t codes) {
   uint32_t h[4];
   asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
       " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
@@ -167,18 +257,23 @@ __device__ __forceinline__ void values4(float (&v)[8], uint32_t codes) {
       : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
       : "r"(codes));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
+  for (int i = 0; i < 4; ++i)
+    v[i] = unpack2<SBC_F16>(h[i]);
 }
 
-/// The values (before the scale) of four 8-bit codes.
-__device__ __forceinline__ void values8x4(float *v, uint32_t w) {
+/// The values of eight 8-bit codes with their scale: code + 128 in the last
+/// bits of 2^23 + 128 + code, again without a conversion instruction. The
+/// product and the difference are exact (a NaN scale gives NaN; an infinite
+/// offset cannot arise, 2^(s-6) being at most 2^121).
+__device__ __forceinline__ void values8(float2 (&v)[4], uint2 codes, float scale) {
+  const uint32_t w[2] = {codes.x ^ 0x80808080u, codes.y ^ 0x80808080u};
+  const float offset = -8388736.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    v[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i)));
+  for (int i = 0; i < 4; ++i) {
+    const float2 b = make_float2(__uint_as_float(__byte_perm(w[i / 2], 0x4b000000u, 0x7440 + (2 * i & 3))),
+                                 __uint_as_float(__byte_perm(w[i / 2], 0x4b000000u, 0x7440 + (2 * i + 1 & 3))));
+    v[i] = __fmul2_rn(__fadd2_rn(b, make_float2(offset, offset)), make_float2(scale, scale));
+  }
 }
 
 } // namespace mx

@@ -124,7 +124,7 @@ int sb_mx_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols, int
   if (on.rc())
     return status(err, "set device", on.rc());
   return status(err, "quantize",
-                sbc_mx_quantize(x, dtype, rows, cols, row_stride, C(along), C(across), nullptr, 0, stream));
+                sbc_mx_quantize(x, dtype, rows, cols, row_stride, C(along), C(across), stream));
 }
 
 int sb_mx_dequantize(const sb_mx *q, void *out, int32_t dtype, int32_t transpose, void *stream, sb_error *err) {
@@ -142,22 +142,7 @@ int sb_mx_dequantize(const sb_mx *q, void *out, int32_t dtype, int32_t transpose
   return status(err, "dequantize", sbc_mx_dequantize(C(q), out, dtype, transpose, stream));
 }
 
-int sb_mx_workspace(int64_t m, int64_t n, int64_t k, int32_t quantize, int32_t device, int64_t *bytes, sb_error *err) {
-  if (m <= 0 || n <= 0 || k <= 0 || !bytes)
-    return fail(err, "invalid_view", "extents are at least 1");
-  OnDevice on(device);
-  if (on.rc())
-    return status(err, "set device", on.rc());
-  if (const int rc = sbc_mx_product_workspace(m, n, k, bytes))
-    return status(err, "workspace", rc);
-  *bytes = up256(*bytes);
-  if (quantize)
-    *bytes += up256(code_bytes(m, k)) + scale_bytes(m, k);
-  return 0;
-}
-
-int sb_mx_matmul(const sb_mx *a, const sb_mx *b, void *y, int32_t dtype, void *workspace, int64_t workspace_bytes,
-                 void *stream, sb_error *err) {
+int sb_mx_matmul(const sb_mx *a, const sb_mx *b, void *y, int32_t dtype, void *stream, sb_error *err) {
   for (const sb_mx *q : {a, b})
     if (const char *w = wrong(q))
       return fail(err, "invalid_view", w);
@@ -174,14 +159,19 @@ int sb_mx_matmul(const sb_mx *a, const sb_mx *b, void *y, int32_t dtype, void *w
   OnDevice on(a->device);
   if (on.rc())
     return status(err, "set device", on.rc());
-  int64_t need = 0;
-  if (const int rc = sbc_mx_product_workspace(a->rows, b->rows, a->cols, &need))
-    return status(err, "workspace", rc);
-  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < need)
-    return fail(err, "insufficient_capacity", "the workspace is smaller than sb_mx_workspace asks for, or not aligned");
   if (earlier_fault(err))
     return 1;
-  return status(err, "matmul", sbc_mx_product(C(a), C(b), y, dtype, workspace, 0, stream));
+  return status(err, "matmul", sbc_mx_product(C(a), nullptr, 0, 0, C(b), y, dtype, 0, stream));
+}
+
+int sb_mx_linear_workspace(int64_t rows, int64_t n, int64_t k, int32_t device, int64_t *bytes, sb_error *err) {
+  if (rows <= 0 || n <= 0 || k <= 0 || !bytes || rows > (int64_t{1} << 56) / k)
+    return fail(err, "invalid_view", "extents are at least 1");
+  OnDevice on(device);
+  if (on.rc())
+    return status(err, "set device", on.rc());
+  *bytes = sbc_mx_fuses_quantize(rows, n, k) ? 0 : up256(code_bytes(rows, k)) + scale_bytes(rows, k);
+  return 0;
 }
 
 int sb_mx_linear(const void *x, int32_t x_dtype, int64_t rows, int64_t row_stride, const sb_mx *weight, void *y,
@@ -190,30 +180,27 @@ int sb_mx_linear(const void *x, int32_t x_dtype, int64_t rows, int64_t row_strid
     return fail(err, "invalid_view", w);
   if (weight->format != SBC_MXFP4)
     return fail(err, "typed_unsupported", "products are those of mxfp4 matrices");
-  if (!x || !y || rows <= 0 || row_stride < 0)
+  if (!x || !y || rows <= 0 || row_stride < 0 || rows > (int64_t{1} << 56) / weight->cols)
     return fail(err, "invalid_view", "x needs at least one row, and rows no less than 0 apart; y is needed");
   if (!known(x_dtype) || !known(y_dtype))
     return fail(err, "typed_unsupported", "values are float32, float16 or bfloat16");
   OnDevice on(weight->device);
   if (on.rc())
     return status(err, "set device", on.rc());
-  const int64_t k = weight->cols;
-  int64_t need = 0;
-  if (const int rc = sbc_mx_product_workspace(rows, weight->rows, k, &need))
-    return status(err, "workspace", rc);
-  need = up256(need);
-  const int64_t codes = up256(code_bytes(rows, k)), scales = scale_bytes(rows, k);
-  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < need + codes + scales)
-    return fail(err, "insufficient_capacity", "the workspace is smaller than sb_mx_workspace asks for, or not aligned");
   if (earlier_fault(err))
     return 1;
-  auto *at = static_cast<uint8_t *>(workspace) + need;
-  const sbc_mx q{at, at + codes, rows, k, SBC_MXFP4, weight->device};
-  const int rc = sbc_mx_quantize(x, x_dtype, rows, k, row_stride, &q, nullptr, static_cast<uint32_t *>(workspace),
-                                 sbc_mx_product_clear_words(rows, weight->rows, k), stream);
-  if (rc)
+  const int64_t k = weight->cols;
+  sbc_mx q{nullptr, nullptr, rows, k, SBC_MXFP4, weight->device};
+  if (sbc_mx_fuses_quantize(rows, weight->rows, k))
+    return status(err, "linear", sbc_mx_product(&q, x, x_dtype, row_stride, C(weight), y, y_dtype, 0, stream));
+  const int64_t codes = up256(code_bytes(rows, k)), scales = scale_bytes(rows, k);
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < codes + scales)
+    return fail(err, "insufficient_capacity", "the workspace is smaller than sb_mx_linear_workspace asks for, or not aligned");
+  q.codes = workspace;
+  q.scales = static_cast<uint8_t *>(workspace) + codes;
+  if (const int rc = sbc_mx_quantize(x, x_dtype, rows, k, row_stride, &q, nullptr, stream))
     return status(err, "quantize", rc);
-  return status(err, "matmul", sbc_mx_product(&q, C(weight), y, y_dtype, workspace, 1, stream));
+  return status(err, "linear", sbc_mx_product(&q, nullptr, 0, 0, C(weight), y, y_dtype, 1, stream));
 }
 
 int sb_silu_mul(const void *gate, int64_t gate_stride, const void *up, int64_t up_stride, int32_t dtype, int64_t rows,

@@ -60,7 +60,7 @@ def _check(rc):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _blocks(cols):
@@ -242,10 +242,10 @@ def dequantize(q, dtype=torch.float16, *, transpose=False):
 
 
 @lru_cache(maxsize=4096)
-def _workspace(m, n, k, quantize, device):
-    bytes_ = ctypes.c_int64()
-    _check(_native.lib().sb_mx_workspace(m, n, k, quantize, device, ctypes.byref(bytes_), _scratch.ref))
-    return bytes_.value
+def _linear_workspace(m, n, k, device):
+    size = ctypes.c_int64()
+    _check(_native.lib().sb_mx_linear_workspace(m, n, k, device, ctypes.byref(size), _scratch.ref))
+    return size.value
 
 
 def matmul(a, b, *, dtype=torch.bfloat16):
@@ -260,10 +260,8 @@ def matmul(a, b, *, dtype=torch.bfloat16):
         raise ValueError(f"a [m, k] and b [n, k] need the same k: got {k} and {kb}")
     y = torch.empty((m, n), dtype=dtype, device=a.device)
     if m and n:
-        size = _workspace(m, n, k, 0, a.device.index)
-        space = torch.empty(size, dtype=torch.uint8, device=a.device)
-        _check(_native.lib().sb_mx_matmul(a.native, b.native, y.data_ptr(), _DTYPES[dtype], space.data_ptr(), size,
-                                          _stream(a.device), _scratch.ref))
+        _check(_native.lib().sb_mx_matmul(a.native, b.native, y.data_ptr(), _DTYPES[dtype], _stream(a.device),
+                                          _scratch.ref))
     return y
 
 
@@ -273,10 +271,11 @@ def _linear(x, w, dtype):
     n = w.shape[0]
     y = torch.empty((*lead, n), dtype=dtype, device=x.device)
     if m and n:
-        size = _workspace(m, n, k, 1, x.device.index)
-        space = torch.empty(size, dtype=torch.uint8, device=x.device)
+        size = _linear_workspace(m, n, k, x.device.index)
+        space = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
         _check(_native.lib().sb_mx_linear(x.data_ptr(), _DTYPES[x.dtype], m, stride, w.native, y.data_ptr(),
-                                          _DTYPES[dtype], space.data_ptr(), size, _stream(x.device), _scratch.ref))
+                                          _DTYPES[dtype], space.data_ptr() if size else None, size,
+                                          _stream(x.device), _scratch.ref))
     return y
 
 

@@ -87,16 +87,16 @@ def test_native_calls_refuse_before_they_launch():
     for bad in (q(codes=0), q(codes=4100), q(scales=8), q(rows=0), q(cols=-1), q(format=7), q(device=-1),
                 q(rows=1 << 41), q(rows=1 << 39, cols=1 << 39)):
         assert _native_call("sb_mx_dequantize", bad, 4096, 0, 0, None) == (1, "invalid_view")
-        assert _native_call("sb_mx_matmul", good, bad, 4096, 0, 4096, 1 << 40, None) == (1, "invalid_view")
+        assert _native_call("sb_mx_matmul", good, bad, 4096, 0, None) == (1, "invalid_view")
         assert _native_call("sb_mx_linear", 4096, 0, 1, 64, bad, 4096, 0, 4096, 1 << 40, None) == (1, "invalid_view")
         assert _native_call("sb_mx_quantize", 4096, 0, 4, 64, 64, bad, None, None) == (1, "invalid_view")
     assert _native_call("sb_mx_dequantize", None, 4096, 0, 0, None) == (1, "invalid_view")
     assert _native_call("sb_mx_dequantize", good, None, 0, 0, None) == (1, "invalid_view")
     assert _native_call("sb_mx_dequantize", good, 4096, 3, 0, None) == (1, "typed_unsupported")
     assert _native_call("sb_mx_dequantize", q(format=1), 4096, 0, 1, None) == (1, "typed_unsupported")
-    assert _native_call("sb_mx_matmul", good, q(cols=32), 4096, 0, 4096, 1 << 40, None) == (1, "invalid_view")
-    assert _native_call("sb_mx_matmul", good, q(device=1), 4096, 0, 4096, 1 << 40, None) == (1, "device_mismatch")
-    assert _native_call("sb_mx_matmul", q(format=1), good, 4096, 0, 4096, 1 << 40, None) == (1, "typed_unsupported")
+    assert _native_call("sb_mx_matmul", good, q(cols=32), 4096, 0, None) == (1, "invalid_view")
+    assert _native_call("sb_mx_matmul", good, q(device=1), 4096, 0, None) == (1, "device_mismatch")
+    assert _native_call("sb_mx_matmul", q(format=1), good, 4096, 0, None) == (1, "typed_unsupported")
     assert _native_call("sb_mx_quantize", 4096, 0, 4, 64, 64, None, None, None) == (1, "invalid_options")
     assert _native_call("sb_mx_quantize", 4096, 0, 5, 64, 64, good, None, None) == (1, "invalid_view")
     assert _native_call("sb_mx_quantize", 4096, 0, 4, 64, -1, good, None, None) == (1, "invalid_view")
