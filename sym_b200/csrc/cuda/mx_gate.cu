@@ -7,8 +7,8 @@
 //
 // Bound by memory: for 16-bit values the forward pass reads 4 bytes per
 // element and writes 2 + 2.06, the backward pass the same the other way
-// round. A block of threads takes 16 rows x 128 columns per unit, a thread 8
-// elements of a row, four lanes a block of 32.
+// round. A block of threads takes 32 rows x 128 columns, a thread 16 values of
+// a row (8 of 32 bits, of two rows), two (four) lanes a block of 32.
 #include "barriers.h"
 #include "mx_values.h"
 
@@ -18,7 +18,8 @@ using namespace mx;
 
 constexpr int kThreads = 256;
 constexpr int kTile = 128;
-constexpr int kUnits = 2; // rows (16 apart) per thread
+constexpr int kRows = 32;
+constexpr uint32_t kMaxY = 32768; // row tiles along the grid's y
 
 struct GateArgs {
   const void *gate, *up; // forward: inputs; backward: `gate` is dh
@@ -26,7 +27,6 @@ struct GateArgs {
   int64_t gate_stride, up_stride, h_stride, dup_stride;
   uint8_t *gate_codes, *gate_scales, *up_codes, *up_scales;
   int64_t rows, cols, blocks;
-  uint32_t tiles_c;
 };
 
 /// 1 / (1 + exp(-g)) from exp(-|g|), which cannot overflow: far below zero the
@@ -44,7 +44,7 @@ template <int DT> __device__ __forceinline__ float sigmoid(float g) {
   }
   const float e = exp2f(fmaf(a, 1.44269502f, a * 1.92596303e-8f));
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e)); // of a normal number
   return (g < 0.f ? e : 1.f) * r;
 }
 
@@ -52,54 +52,84 @@ template <int DT> __device__ __forceinline__ float2 sigmoid2(float2 g) {
   return make_float2(sigmoid<DT>(g.x), sigmoid<DT>(g.y));
 }
 
-/// Keep eight values of one block quarter in 8 bits.
+/// Keep a part's values in 8 bits.
 template <int DT>
-__device__ __forceinline__ void keep8(uint8_t *codes, uint8_t *scales, const Raw8<DT> &raw, const float2 (&v)[4],
-                                      int64_t block, int quarter, bool exists) {
-  const uint32_t byte = scale_byte<SBC_MXINT8>(top_of_lanes<2>(raw.top()));
-  uint2 w = codes8(v, inverse_scale<SBC_MXINT8>(byte));
-  if (byte == 255)
-    w = make_uint2(0, 0);
+__device__ __forceinline__ void keep(uint8_t *codes, uint8_t *scales, const Part<DT> &in, int64_t block, int at,
+                                     bool exists) {
+  constexpr int N = Part<DT>::kValues / 8;
+  const uint32_t byte = scale_byte<SBC_MXINT8>(in.block_top());
+  const float inv = inverse_scale<SBC_MXINT8>(byte);
+  uint2 w[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float2 v[4];
+    in.raw[i].values(v);
+    w[i] = codes8(v, inv);
+    if (byte == 255)
+      w[i] = make_uint2(0, 0);
+  }
   if (exists) {
-    __stcs(reinterpret_cast<uint2 *>(codes + block * 32 + quarter * 8), w);
-    if (quarter == 0)
+    if (N == 2)
+      __stcs(reinterpret_cast<uint4 *>(codes + block * 32 + at), make_uint4(w[0].x, w[0].y, w[N - 1].x, w[N - 1].y));
+    else
+      __stcs(reinterpret_cast<uint2 *>(codes + block * 32 + at), w[0]);
+    if (at == 0)
       scales[block] = static_cast<uint8_t>(byte);
   }
 }
 
+/// Where a thread works: row r0 (and kStride on), column c, `cols` of its values
+/// existing.
+template <int DT> struct Place {
+  static constexpr int kStride = kThreads / Part<DT>::kLanes, kUnits = kRows / kStride;
+  int64_t r0, c;
+  int cols, in_block;
+  __device__ __forceinline__ explicit Place(const GateArgs &a) {
+    r0 = (static_cast<int64_t>(blockIdx.z) * kMaxY + blockIdx.y) * kRows + threadIdx.x / Part<DT>::kLanes;
+    c = static_cast<int64_t>(blockIdx.x) * kTile + threadIdx.x % Part<DT>::kLanes * Part<DT>::kValues;
+    const int64_t left = a.cols - c;
+    cols = static_cast<int>(left < 0 ? 0 : left < Part<DT>::kValues ? left : Part<DT>::kValues);
+    in_block = static_cast<int>(c % kBlock);
+  }
+};
+
 template <int DT, bool KEEP, bool VEC>
-__global__ void __launch_bounds__(kThreads) k_silu_mul(const __grid_constant__ GateArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) k_silu_mul(const __grid_constant__ GateArgs a) {
   using T = typename Value<DT>::T;
-  const uint32_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x - tr * a.tiles_c;
-  const int64_t r0 = static_cast<int64_t>(tr) * (16 * kUnits) + (threadIdx.x >> 4);
-  const int64_t c = static_cast<int64_t>(tc) * kTile + (threadIdx.x & 15) * 8;
-  const int cols = static_cast<int>(a.cols - c < 0 ? 0 : a.cols - c < 8 ? a.cols - c : 8);
-  const T *gate_at = static_cast<const T *>(a.gate) + r0 * a.gate_stride + c;
-  const T *up_at = static_cast<const T *>(a.up) + r0 * a.up_stride + c;
-  T *h_at = static_cast<T *>(a.h) + r0 * a.cols + c;
-  const int64_t block = r0 * a.blocks + c / kBlock;
-  Raw8<DT> gate[kUnits], up[kUnits];
+  using P = Place<DT>;
+  constexpr int N = Part<DT>::kValues / 8;
+  const P p(a);
+  const T *gate_at = static_cast<const T *>(a.gate) + p.r0 * a.gate_stride + p.c;
+  const T *up_at = static_cast<const T *>(a.up) + p.r0 * a.up_stride + p.c;
+  T *h_at = static_cast<T *>(a.h) + p.r0 * a.cols + p.c;
+  const int64_t block = p.r0 * a.blocks + p.c / kBlock;
+  Part<DT> gate[P::kUnits], up[P::kUnits];
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
-    const int have = r0 + 16 * i < a.rows ? cols : 0;
-    gate[i].template load<VEC>(gate_at + 16 * i * a.gate_stride, have);
-    up[i].template load<VEC>(up_at + 16 * i * a.up_stride, have);
+  for (int i = 0; i < P::kUnits; ++i) {
+    const int have = p.r0 + P::kStride * i < a.rows ? p.cols : 0;
+    gate[i].template load<VEC>(gate_at + P::kStride * i * a.gate_stride, have);
+    up[i].template load<VEC>(up_at + P::kStride * i * a.up_stride, have);
   }
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
-    float2 g[4], u[4], h[4];
-    gate[i].values(g);
-    up[i].values(u);
+  for (int i = 0; i < P::kUnits; ++i) {
+    float2 h[N][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      h[k] = __fmul2_rn(__fmul2_rn(g[k], sigmoid2<DT>(g[k])), u[k]);
-    const bool row_exists = r0 + 16 * i < a.rows;
+    for (int j = 0; j < N; ++j) {
+      float2 g[4], u[4];
+      gate[i].raw[j].values(g);
+      up[i].raw[j].values(u);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        h[j][k] = __fmul2_rn(__fmul2_rn(g[k], sigmoid2<DT>(g[k])), u[k]);
+    }
+    const bool row_exists = p.r0 + P::kStride * i < a.rows;
     if (row_exists)
-      store8<DT, VEC>(h_at + 16 * i * a.cols, h, cols);
+      store_part<DT, VEC>(h_at + P::kStride * i * a.cols, h, p.cols);
     if (KEEP) {
-      const bool exists = row_exists && c < a.blocks * kBlock;
-      keep8(a.gate_codes, a.gate_scales, gate[i], g, block + 16 * i * a.blocks, threadIdx.x & 3, exists);
-      keep8(a.up_codes, a.up_scales, up[i], u, block + 16 * i * a.blocks, threadIdx.x & 3, exists);
+      const bool exists = row_exists && p.c < a.blocks * kBlock;
+      const int64_t at = block + P::kStride * i * a.blocks;
+      keep<DT>(a.gate_codes, a.gate_scales, gate[i], at, p.in_block, exists);
+      keep<DT>(a.up_codes, a.up_scales, up[i], at, p.in_block, exists);
     }
   }
 }
@@ -107,47 +137,61 @@ __global__ void __launch_bounds__(kThreads) k_silu_mul(const __grid_constant__ G
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_silu_mul_backward(const __grid_constant__ GateArgs a) {
   using T = typename Value<DT>::T;
-  const uint32_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x - tr * a.tiles_c;
-  const int64_t r0 = static_cast<int64_t>(tr) * (16 * kUnits) + (threadIdx.x >> 4);
-  const int64_t c = static_cast<int64_t>(tc) * kTile + (threadIdx.x & 15) * 8;
-  const int cols = static_cast<int>(a.cols - c < 8 ? a.cols - c : 8);
-  if (cols <= 0)
+  using P = Place<DT>;
+  constexpr int N = Part<DT>::kValues / 8;
+  const P p(a);
+  if (p.cols <= 0)
     return;
-  Raw8<DT> in[kUnits];
-  uint2 gate[kUnits], up[kUnits];
-  uint32_t gate_scale[kUnits], up_scale[kUnits];
-  const T *dh_at = static_cast<const T *>(a.gate) + r0 * a.gate_stride + c;
-  const int64_t block0 = r0 * a.blocks + c / kBlock;
+  Part<DT> in[P::kUnits];
+  uint2 gate[P::kUnits][N], up[P::kUnits][N];
+  uint32_t gate_scale[P::kUnits], up_scale[P::kUnits];
+  const T *dh_at = static_cast<const T *>(a.gate) + p.r0 * a.gate_stride + p.c;
+  const int64_t block0 = p.r0 * a.blocks + p.c / kBlock;
+  const auto codes = [](uint2 (&w)[N], const uint8_t *at) {
+    if (N == 2) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4 *>(at));
+      w[0] = make_uint2(q.x, q.y);
+      w[N - 1] = make_uint2(q.z, q.w);
+    } else {
+      w[0] = __ldg(reinterpret_cast<const uint2 *>(at));
+    }
+  };
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
-    const int64_t block = block0 + 16 * i * a.blocks, at = block * 32 + (threadIdx.x & 3) * 8;
-    if (r0 + 16 * i < a.rows) {
-      in[i].template load<VEC>(dh_at + 16 * i * a.gate_stride, cols);
-      gate[i] = __ldg(reinterpret_cast<const uint2 *>(a.gate_codes + at));
-      up[i] = __ldg(reinterpret_cast<const uint2 *>(a.up_codes + at));
+  for (int i = 0; i < P::kUnits; ++i) {
+    if (p.r0 + P::kStride * i < a.rows) {
+      const int64_t block = block0 + P::kStride * i * a.blocks;
+      in[i].template load<VEC>(dh_at + P::kStride * i * a.gate_stride, p.cols);
+      codes(gate[i], a.gate_codes + block * 32 + p.in_block);
+      codes(up[i], a.up_codes + block * 32 + p.in_block);
       gate_scale[i] = __ldg(a.gate_scales + block);
       up_scale[i] = __ldg(a.up_scales + block);
     }
   }
-  T *dgate_at = static_cast<T *>(a.h) + r0 * a.h_stride + c, *dup_at = static_cast<T *>(a.dup) + r0 * a.dup_stride + c;
+  T *dgate_at = static_cast<T *>(a.h) + p.r0 * a.h_stride + p.c;
+  T *dup_at = static_cast<T *>(a.dup) + p.r0 * a.dup_stride + p.c;
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
-    if (r0 + 16 * i >= a.rows)
+  for (int i = 0; i < P::kUnits; ++i) {
+    if (p.r0 + P::kStride * i >= a.rows)
       return;
-    float2 dh[4], g[4], u[4], dg[4], du[4];
-    in[i].values(dh);
-    values8(g, gate[i], scale_value<SBC_MXINT8>(gate_scale[i]));
-    values8(u, up[i], scale_value<SBC_MXINT8>(up_scale[i]));
+    const float gs = scale_value<SBC_MXINT8>(gate_scale[i]), us = scale_value<SBC_MXINT8>(up_scale[i]);
     const float2 one = make_float2(1.f, 1.f);
+    float2 dg[N][4], du[N][4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 s = sigmoid2<DT>(g[k]);
-      const float2 rest = __fadd2_rn(one, make_float2(-s.x, -s.y));
-      dg[k] = __fmul2_rn(__fmul2_rn(dh[k], u[k]), __fmul2_rn(s, __ffma2_rn(g[k], rest, one)));
-      du[k] = __fmul2_rn(dh[k], __fmul2_rn(g[k], s));
+    for (int j = 0; j < N; ++j) {
+      float2 dh[4], g[4], u[4];
+      in[i].raw[j].values(dh);
+      values8(g, gate[i][j], gs);
+      values8(u, up[i][j], us);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 s = sigmoid2<DT>(g[k]);
+        const float2 rest = __fadd2_rn(one, make_float2(-s.x, -s.y));
+        dg[j][k] = __fmul2_rn(__fmul2_rn(dh[k], u[k]), __fmul2_rn(s, __ffma2_rn(g[k], rest, one)));
+        du[j][k] = __fmul2_rn(dh[k], __fmul2_rn(g[k], s));
+      }
     }
-    store8<DT, VEC>(dgate_at + 16 * i * a.h_stride, dg, cols);
-    store8<DT, VEC>(dup_at + 16 * i * a.dup_stride, du, cols);
+    store_part<DT, VEC>(dgate_at + P::kStride * i * a.h_stride, dg, p.cols);
+    store_part<DT, VEC>(dup_at + P::kStride * i * a.dup_stride, du, p.cols);
   }
 }
 
@@ -155,21 +199,20 @@ bool aligned(const void *p, int64_t stride, int width) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * width % 16 == 0;
 }
 
-bool shape(GateArgs &a, int64_t rows, int64_t cols, unsigned *grid) {
+bool shape(GateArgs &a, int64_t rows, int64_t cols, dim3 *grid) {
   if (rows <= 0 || cols <= 0)
     return false;
   a.rows = rows;
   a.cols = cols;
   a.blocks = blocks_of(cols);
-  const int64_t tc = (cols + kTile - 1) / kTile, n = (rows + 16 * kUnits - 1) / (16 * kUnits) * tc;
-  if (n > INT32_MAX)
+  const int64_t tc = (cols + kTile - 1) / kTile, tr = (rows + kRows - 1) / kRows, z = (tr + kMaxY - 1) / kMaxY;
+  if (tc > INT32_MAX || z > 65535)
     return false;
-  a.tiles_c = static_cast<uint32_t>(tc);
-  *grid = static_cast<unsigned>(n);
+  *grid = dim3(static_cast<unsigned>(tc), static_cast<unsigned>(tr < kMaxY ? tr : kMaxY), static_cast<unsigned>(z));
   return true;
 }
 
-template <int DT> int launch_forward(const GateArgs &a, bool vec, unsigned grid, cudaStream_t s) {
+template <int DT> int launch_forward(const GateArgs &a, bool vec, dim3 grid, cudaStream_t s) {
   const bool keep = a.gate_codes != nullptr;
   auto k = keep ? (vec ? k_silu_mul<DT, true, true> : k_silu_mul<DT, true, false>)
                 : (vec ? k_silu_mul<DT, false, true> : k_silu_mul<DT, false, false>);
@@ -178,7 +221,7 @@ template <int DT> int launch_forward(const GateArgs &a, bool vec, unsigned grid,
   return cudaGetLastError();
 }
 
-template <int DT> int launch_backward(const GateArgs &a, bool vec, unsigned grid, cudaStream_t s) {
+template <int DT> int launch_backward(const GateArgs &a, bool vec, dim3 grid, cudaStream_t s) {
   auto k = vec ? k_silu_mul_backward<DT, true> : k_silu_mul_backward<DT, false>;
   k<<<grid, kThreads, 0, s>>>(a);
   sbc::count_launch();
@@ -192,7 +235,7 @@ extern "C" {
 int sbc_silu_mul(const void *gate, int64_t gate_stride, const void *up, int64_t up_stride, int32_t dtype, int64_t rows,
                  int64_t cols, void *h, const sbc_mx *gate_q, const sbc_mx *up_q, void *stream) {
   GateArgs a{};
-  unsigned grid = 0;
+  dim3 grid;
   if (!gate || !up || !h || !gate_q != !up_q || dtype < SBC_F32 || dtype > SBC_BF16 || !shape(a, rows, cols, &grid))
     return SBC_EINVAL;
   a.gate = gate;
@@ -220,7 +263,7 @@ int sbc_silu_mul(const void *gate, int64_t gate_stride, const void *up, int64_t 
 int sbc_silu_mul_backward(const void *dh, int64_t dh_stride, int32_t dtype, const sbc_mx *gate_q, const sbc_mx *up_q,
                           void *dgate, int64_t dgate_stride, void *dup, int64_t dup_stride, void *stream) {
   GateArgs a{};
-  unsigned grid = 0;
+  dim3 grid;
   if (!dh || !gate_q || !up_q || !dgate || !dup || dtype < SBC_F32 || dtype > SBC_BF16 ||
       gate_q->format != SBC_MXINT8 || up_q->format != SBC_MXINT8 || gate_q->rows != up_q->rows ||
       gate_q->cols != up_q->cols || !shape(a, gate_q->rows, gate_q->cols, &grid))

@@ -21,16 +21,12 @@ struct QuantizeArgs {
   uint32_t tiles_c;
 };
 
-/// Blocks along the columns: a thread holds V = 8 or 16 values of a row, 32 / V
-/// lanes a block (a shuffle each for its largest magnitude). codes and scales
-/// point at this thread's place in the row; `exists`: its block does.
+/// Codes and scale of a thread's part of a block. codes and scales point at
+/// this thread's place in the row; `exists`: its block does.
 template <int DT, int FMT, int V>
-__device__ __forceinline__ void row_unit(const Raw8<DT> (&in)[V / 8], uint8_t *codes, uint8_t *scales, bool exists,
-                                         bool row_exists) {
-  float top = in[0].top();
-  if (V == 16)
-    top = fmaxf_bits(top, in[V / 8 - 1].top());
-  const uint32_t byte = scale_byte<FMT>(top_of_lanes<V == 8 ? 2 : 1>(top));
+__device__ __forceinline__ void quantize_part(const Raw8<DT> (&in)[V / 8], float top, uint8_t *codes, uint8_t *scales,
+                                              bool exists, bool row_exists) {
+  const uint32_t byte = scale_byte<FMT>(top);
   const float inv = inverse_scale<FMT>(byte);
   uint32_t w[FMT == SBC_MXFP4 ? V / 8 : V / 4];
 #pragma unroll
@@ -66,13 +62,11 @@ __device__ __forceinline__ void row_unit(const Raw8<DT> (&in)[V / 8], uint8_t *c
 
 /// Blocks along the columns only: 64 rows (FEW: as many as one unit a thread
 /// covers) x 128 columns per block of threads, the loads of all units before
-/// the first use. 16-bit values go 16 to a thread, which halves the work
-/// per block and per row beside the values' own; with 16 32-bit values the
-/// lanes of a load would lie 64 bytes apart.
+/// the first use.
 template <int DT, int FMT, bool FEW, bool VEC>
 __global__ void __launch_bounds__(kThreads) k_mx_quantize(const __grid_constant__ QuantizeArgs a) {
   using T = typename Value<DT>::T;
-  constexpr int V = DT == SBC_F32 ? 8 : 16, kLanes = kTile / V, kStride = kThreads / kLanes; // rows between units
+  constexpr int V = Part<DT>::kValues, kLanes = Part<DT>::kLanes, kStride = kThreads / kLanes; // rows between units
   constexpr int kUnits = FEW ? 1 : 64 / kStride;
   // A kernel launched to overlap this one's end may begin its own set-up; it
   // waits for this grid's completion before it reads what is written here.
@@ -84,12 +78,10 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize(const __grid_constant_
   const int have = static_cast<int>(left < 0 ? 0 : left < V ? left : V);
   const T *x = static_cast<const T *>(a.x) + r0 * a.row_stride + c;
   const int rows = static_cast<int>(a.rows - r0 < 64 ? a.rows - r0 : 64); // from r0 on
-  Raw8<DT> in[kUnits][V / 8];
+  Part<DT> in[kUnits];
 #pragma unroll
   for (int i = 0; i < kUnits; ++i)
-#pragma unroll
-    for (int j = 0; j < V / 8; ++j)
-      in[i][j].template load<VEC>(x + i * kStride * a.row_stride + 8 * j, i * kStride < rows ? have - 8 * j : 0);
+    in[i].template load<VEC>(x + i * kStride * a.row_stride, i * kStride < rows ? have : 0);
   const int64_t blocks = blocks_of(a.cols);
   const bool exists = c < blocks * kBlock;
   constexpr int kBytes = FMT == SBC_MXFP4 ? 16 : 32; // of codes per block
@@ -102,7 +94,8 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize(const __grid_constant_
     // bytes and one row 16
     const int64_t scale_step = FMT == SBC_MXFP4 ? (i * kStride / 32) * 4 + (i * kStride % 32) * 16 : i * kStride * blocks;
     const bool row_exists = i * kStride < rows;
-    row_unit<DT, FMT, V>(in[i], codes + i * code_step, scales + scale_step, row_exists && exists, row_exists);
+    quantize_part<DT, FMT, V>(in[i].raw, in[i].block_top(), codes + i * code_step, scales + scale_step,
+                              row_exists && exists, row_exists);
   }
 }
 
@@ -114,32 +107,33 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize_across(const __grid_co
   const int t = threadIdx.x;
   const uint32_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x - tr * a.tiles_c;
   const int64_t r0 = static_cast<int64_t>(tr) * kTile, c0 = static_cast<int64_t>(tc) * kTile;
-  const T *x = static_cast<const T *>(a.x);
-  const int c8 = (t & 15) * 8;
-  const int64_t c = c0 + c8;
-  const int have = static_cast<int>(a.cols - c < 0 ? 0 : a.cols - c < 8 ? a.cols - c : 8);
+  constexpr int V = Part<DT>::kValues, kLanes = Part<DT>::kLanes, kStride = kThreads / kLanes, kUnits = kTile / kStride;
+  const int row0 = t / kLanes, c8 = t % kLanes * V;
+  const int64_t c = c0 + c8, left = a.cols - c;
+  const int have = static_cast<int>(left < 0 ? 0 : left < V ? left : V);
   const int here = static_cast<int>(a.rows - r0 < kTile ? a.rows - r0 : kTile);
+  const T *x = static_cast<const T *>(a.x) + (r0 + row0) * a.row_stride + c;
   extern __shared__ uint4 smem[];
   T *tile = reinterpret_cast<T *>(smem);                           // [128][128]
   uint4 *codes = smem + kTile * kTile * sizeof(T) / 16;            // [128 columns][4]
   uint8_t *scales = reinterpret_cast<uint8_t *>(codes + kTile * 4); // [512]
   const int64_t row_blocks = blocks_of(a.cols);
-  uint8_t *row_codes = a.codes + (r0 + (t >> 4)) * row_blocks * 16 + c / 2;
-  uint8_t *row_scales = a.scales + scale_word(r0 + (t >> 4), tc, quads_of(a.cols)) + c8 / 32;
-  Raw8<DT> in[8];
+  uint8_t *row_codes = a.codes + (r0 + row0) * row_blocks * 16 + c / 2;
+  uint8_t *row_scales = a.scales + scale_word(r0 + row0, tc, quads_of(a.cols)) + c8 / 32;
+  Part<DT> in[kUnits];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = (t >> 4) + 16 * i;
-    in[i].template load<VEC>(x + (r0 + row) * a.row_stride + c, row < here ? have : 0);
-  }
+  for (int i = 0; i < kUnits; ++i)
+    in[i].template load<VEC>(x + i * kStride * a.row_stride, row0 + i * kStride < here ? have : 0);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = (t >> 4) + 16 * i;
-    *reinterpret_cast<Raw8<DT> *>(tile + row * kTile + c8) = in[i];
-    if (ROWS && (row & ~1) < here) // the warp's two rows
-      row_unit<DT, SBC_MXFP4, 8>(*reinterpret_cast<const Raw8<DT>(*)[1]>(&in[i]), row_codes + i * (16 * row_blocks * 16),
-                                 row_scales + (i / 2) * 4 + (i % 2) * 256, row < here && c < row_blocks * kBlock,
-                                 row < here);
+  for (int i = 0; i < kUnits; ++i) {
+    const int row = row0 + i * kStride;
+#pragma unroll
+    for (int j = 0; j < V / 8; ++j)
+      *reinterpret_cast<Raw8<DT> *>(tile + row * kTile + c8 + 8 * j) = in[i].raw[j];
+    if (ROWS)
+      quantize_part<DT, SBC_MXFP4, V>(in[i].raw, in[i].block_top(), row_codes + i * (kStride * 16) * row_blocks,
+                                      row_scales + (i * kStride / 32) * 4 + (i * kStride % 32) * 16,
+                                      row < here && c < row_blocks * kBlock, row < here);
   }
   __syncthreads();
   // Blocks along the rows: a thread takes 32 rows of two neighbouring 16-bit
@@ -229,7 +223,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const __grid_constan
   const int64_t blocks = blocks_of(a.cols);
   // four 4-bit codes are half a word, which two lanes read
   const uint8_t *codes_at = a.codes + r0 * blocks * kBytes + (c * kBytes / 32 & ~int64_t{3});
-  const int shift = V * kBytes / 32 == 2 ? static_cast<int>(c & 4) * 4 : 0;
+  const bool upper = V * kBytes / 32 == 2 && (c & 4);
   const uint8_t *scales = a.scales + (FMT == SBC_MXFP4 ? scale_word(r0, tc, quads_of(a.cols)) + c8 / 32 : r0 * blocks + c / 32);
   C codes[kUnits];
   uint32_t scale[kUnits];
@@ -248,7 +242,11 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const __grid_constan
     float2 v[4];
     const float s = scale_value<FMT>(scale[i]);
     if constexpr (FMT == SBC_MXFP4) {
-      values4(v, codes[i] >> shift);
+      values4(v, codes[i]); // the whole word, of which four values are this lane's
+      if (V == 4 && upper) {
+        v[0] = v[2];
+        v[1] = v[3];
+      }
       times(v, s);
     } else {
       uint2 w = make_uint2(0, 0);
@@ -281,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const __grid_constan
 /// A block takes every gridDim-th tile; the next tile's codes and scales are
 /// on their way to registers while this one's values are stored.
 template <int DT, bool VEC>
-__global__ void __launch_bounds__(kThreads) k_mx_dequantize_t(const __grid_constant__ DequantizeArgs a) {
+__global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 3 : 4) k_mx_dequantize_t(const __grid_constant__ DequantizeArgs a) {
   using T = typename Value<DT>::T;
   constexpr int kPitch = 18;
   __shared__ uint32_t codes[2][kTile * kPitch];
@@ -325,23 +323,32 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize_t(const __grid_const
     const int have = static_cast<int>(a.rows - r < 8 ? a.rows - r : 8);
     if (have <= 0 || c0 + 8 * c >= a.cols)
       continue;
-    // what was staged for rows past the end is never stored
-    float2 v[8][4];
+    // Two columns at a time from the codes' 16-bit values, which keeps the
+    // registers of four blocks to an SM. What was staged for rows past the end
+    // is never stored.
+    uint32_t h[8][4];
+    float scale[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      values4(v[i], codes[buf][(16 * i + ag) * kPitch + c]);
-      times(v[i], scale_value<SBC_MXFP4>(scales[buf][8 * ag + i] >> (c >> 2) * 8 & 255));
+      pairs4(h[i], codes[buf][(16 * i + ag) * kPitch + c]);
+      scale[i] = scale_value<SBC_MXFP4>(scales[buf][8 * ag + i] >> (c >> 2) * 8 & 255);
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (c0 + 8 * c + j >= a.cols)
-        break;
-      float2 col[4];
+    for (int j = 0; j < 4; ++j) {
+      float2 two[8]; // columns 2 j and 2 j + 1 of eight rows
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        col[i] = j & 1 ? make_float2(v[2 * i][j / 2].y, v[2 * i + 1][j / 2].y)
-                       : make_float2(v[2 * i][j / 2].x, v[2 * i + 1][j / 2].x);
-      store8<DT, VEC>(static_cast<T *>(a.out) + (c0 + 8 * c + j) * a.rows + r, col, have);
+      for (int i = 0; i < 8; ++i)
+        two[i] = __fmul2_rn(unpack2<SBC_F16>(h[i][j]), make_float2(scale[i], scale[i]));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (c0 + 8 * c + 2 * j + k >= a.cols)
+          break;
+        float2 col[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          col[i] = k ? make_float2(two[2 * i].y, two[2 * i + 1].y) : make_float2(two[2 * i].x, two[2 * i + 1].x);
+        store8<DT, VEC>(static_cast<T *>(a.out) + (c0 + 8 * c + 2 * j + k) * a.rows + r, col, have);
+      }
     }
   }
 }
@@ -364,10 +371,11 @@ template <int DT, bool VEC> int launch_quantize(const QuantizeArgs &a, int fmt, 
     k<<<grid, kThreads, 0, s>>>(a);
   } else {
     const int bytes = kTile * kTile * static_cast<int>(sizeof(typename Value<DT>::T)) + kTile * 64 + 512;
-    auto k = a.codes ? k_mx_quantize_across<DT, true, VEC> : k_mx_quantize_across<DT, false, VEC>;
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const cudaError_t e = a.codes ? sbc::allow_shared<k_mx_quantize_across<DT, true, VEC>>()
+                                  : sbc::allow_shared<k_mx_quantize_across<DT, false, VEC>>();
     if (e != cudaSuccess)
       return e;
+    auto k = a.codes ? k_mx_quantize_across<DT, true, VEC> : k_mx_quantize_across<DT, false, VEC>;
     k<<<grid, kThreads, bytes, s>>>(a);
   }
   sbc::count_launch();
@@ -435,8 +443,16 @@ int sbc_mx_dequantize(const sbc_mx *q, void *out, int32_t dtype, int32_t transpo
       dtype > SBC_BF16 || !grid_of(q->rows, q->cols, transpose ? kTile : few ? (dtype == SBC_F32 ? 8 : 16) : 64, &a.tiles_c, &grid))
     return SBC_EINVAL;
   a.tiles = grid;
-  if (transpose && grid > 148 * 3) // three blocks stay on each SM
-    grid = 148 * 3;
+  if (transpose) { // the blocks that stay on the SMs
+    int device = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess)
+      e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess)
+      return e;
+    const uint32_t stay = static_cast<uint32_t>(sms) * (dtype == SBC_F32 ? 3 : 4);
+    grid = grid < stay ? grid : stay;
+  }
   a.codes = static_cast<const uint8_t *>(q->codes);
   a.scales = static_cast<const uint8_t *>(q->scales);
   a.out = out;

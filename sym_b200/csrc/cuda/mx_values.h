@@ -139,11 +139,6 @@ template <int DT> struct Raw8 {
   }
 };
 
-/// The larger of two magnitudes, a NaN above all.
-__device__ __forceinline__ float fmaxf_bits(float a, float b) {
-  return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
-}
-
 /// The largest magnitude over the 2^n lanes of a block's quarters; magnitudes
 /// and NaN order like their bits.
 template <int N> __device__ __forceinline__ float top_of_lanes(float m) {
@@ -179,6 +174,58 @@ __device__ __forceinline__ void store8(typename Value<DT>::T *p, const float2 (&
     for (int i = 0; i < 8; ++i)
       if (i < have)
         u[i] = DT == SBC_F32 ? static_cast<U>(w[i & 7]) : static_cast<U>(w[i >> 1] >> (i & 1) * 16);
+  }
+}
+
+/// V values of a row, V = 8 or (16-bit types) 16: a thread's share of a block,
+/// so that a block's own work is shared by 32 / V lanes. Sixteen lie in one
+/// 32-byte sector, taken by one instruction where it is aligned to that.
+template <int DT> struct Part {
+  static constexpr int kValues = DT == SBC_F32 ? 8 : 16;
+  static constexpr int kLanes = 128 / kValues; // per 128 columns
+  Raw8<DT> raw[kValues / 8];
+
+  template <bool VEC> __device__ __forceinline__ void load(const typename Value<DT>::T *p, int have) {
+    if (VEC && have >= kValues && reinterpret_cast<uintptr_t>(p) % 32 == 0) {
+      uint32_t *w = reinterpret_cast<uint32_t *>(raw);
+      asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "l"(p));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kValues / 8; ++i)
+        raw[i].template load<VEC>(p + 8 * i, have - 8 * i);
+    }
+  }
+
+  /// Largest magnitude of the block, from the lanes that share it.
+  __device__ __forceinline__ float block_top() const {
+    float top = raw[0].top();
+    if (kValues == 16)
+      top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(raw[kValues / 8 - 1].top())));
+    return top_of_lanes<kValues == 8 ? 2 : 1>(top);
+  }
+};
+
+/// Stores a part's values, of which `have` exist.
+template <int DT, bool VEC>
+__device__ __forceinline__ void store_part(typename Value<DT>::T *p, const float2 (&v)[Part<DT>::kValues / 8][4], int have) {
+  constexpr int V = Part<DT>::kValues;
+  if (VEC && have >= V && reinterpret_cast<uintptr_t>(p) % 32 == 0) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (DT == SBC_F32)
+        w[i] = __float_as_uint(i & 1 ? v[0][i / 2].y : v[0][i / 2].x);
+      else
+        w[i] = pack2<DT>(v[i / 4 % (V / 8)][i & 3].x, v[i / 4 % (V / 8)][i & 3].y);
+    asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 8; ++i)
+      store8<DT, VEC>(p + 8 * i, v[i], have - 8 * i);
   }
 }
 
@@ -248,14 +295,21 @@ __device__ __forceinline__ uint2 codes8(const float2 (&v)[4], float inv) {
                     __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410));
 }
 
-/// The values (before the scale) of eight 4-bit codes.
-__device__ __forceinline__ void values4(float2 (&v)[4], uint32_t codes) {
-  uint32_t h[4];
+/// The values (before the scale) of eight 4-bit codes, as pairs of 16-bit floats.
+/// All four pairs are to be used: with this compiler (12.9) the conversions gave
+/// zeros where the upper pairs were not and the upper codes known to be zero.
+__device__ __forceinline__ void pairs4(uint32_t (&h)[4], uint32_t codes) {
   asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
       " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
       " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
       : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
       : "r"(codes));
+}
+
+/// The same in 32 bits.
+__device__ __forceinline__ void values4(float2 (&v)[4], uint32_t codes) {
+  uint32_t h[4];
+  pairs4(h, codes);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     v[i] = unpack2<SBC_F16>(h[i]);

@@ -59,12 +59,27 @@ def _check(rc):
         _raise_transfer(_scratch.error)
 
 
-def _stream(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _stream(index):
+    """The current stream (a cudaStream_t) of a device."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+_library = None
+
+
+def _lib():
+    global _library
+    if _library is None:
+        _library = _native.lib()
+    return _library
 
 
 def _blocks(cols):
     return -(-cols // BLOCK)
+
+
+def _up256(n):
+    return -(-n // 256) * 256
 
 
 def _scale_bytes(rows, cols, format):
@@ -107,10 +122,16 @@ class MxTensor:
                                        codes.device.index)
 
     @classmethod
-    def empty(cls, rows, cols, device, format="mxfp4"):
-        codes = torch.empty((rows, _blocks(cols) * _CODE_BYTES[format]), dtype=torch.uint8, device=device)
-        scales = torch.empty(_scale_bytes(rows, cols, format), dtype=torch.uint8, device=device)
-        return cls(codes, scales, (rows, cols), format)
+    def _empty(cls, like, rows, cols, format="mxfp4"):
+        """An uninitialised matrix on the device of ``like``."""
+        q = cls.__new__(cls)
+        q.codes = like.new_empty((rows, _blocks(cols) * _CODE_BYTES[format]), dtype=torch.uint8)
+        q.scales = like.new_empty(_scale_bytes(rows, cols, format), dtype=torch.uint8)
+        q.shape, q.format, q.native = (rows, cols), format, None
+        if rows:
+            q.native = _native.SbMx(q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, FORMATS[format],
+                                    like.get_device())
+        return q
 
     @classmethod
     def from_rows(cls, codes, row_scales, cols, format="mxfp4"):
@@ -136,6 +157,9 @@ class MxTensor:
     def device(self):
         return self.codes.device
 
+    def get_device(self):
+        return self.codes.get_device()
+
     def to(self, device, non_blocking=False):
         return MxTensor(self.codes.to(device, non_blocking=non_blocking),
                         self.scales.to(device, non_blocking=non_blocking), self.shape, self.format)
@@ -144,11 +168,14 @@ class MxTensor:
         return f"MxTensor({list(self.shape)}, {self.format}, {self.device})"
 
 
-def _matrix(x, name):
+def _matrix(x):
     """x as a matrix whose columns are adjacent: (tensor, rows, cols, row stride)."""
+    cols = x.shape[-1]
+    if x.is_contiguous():
+        return x, x.numel() // cols, cols, cols
     if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
-    rows, cols = x.shape
+        x = x.reshape(-1, cols)
+    rows = x.shape[0]
     if cols > 1 and x.stride(1) != 1:
         x = x.contiguous()
     return x, rows, cols, x.stride(0) if rows > 1 else cols
@@ -167,7 +194,7 @@ def _values(x, name, least=1):
 
 
 def _mx(q, name, format=None):
-    if not isinstance(q, MxTensor):
+    if type(q) is not MxTensor:
         raise TypeError(f"{name} is an MxTensor")
     if not q.codes.is_cuda:
         raise ValueError(f"{name} is on {q.device}: microscaled operators run on CUDA devices")
@@ -184,14 +211,58 @@ def _result(dtype, default):
 
 
 def _quantize(x, format, along, across):
-    x, rows, cols, stride = _matrix(x, "x")
-    q = MxTensor.empty(rows, cols, x.device, format) if along else None
-    qt = MxTensor.empty(cols, rows, x.device) if across else None
+    x, rows, cols, stride = _matrix(x)
+    q = MxTensor._empty(x, rows, cols, format) if along else None
+    qt = MxTensor._empty(x, cols, rows) if across else None
     if rows:
-        _check(_native.lib().sb_mx_quantize(
-            x.data_ptr(), _DTYPES[x.dtype], rows, cols, stride, q.native if along else None,
-            qt.native if across else None, _stream(x.device), _scratch.ref))
+        _check(_lib().sb_mx_quantize(x.data_ptr(), _DTYPES[x.dtype], rows, cols, stride, q.native if along else None,
+                                     qt.native if across else None, _stream(x.get_device()), _scratch.ref))
     return q, qt
+
+
+@lru_cache(maxsize=4096)
+def _layout(*matrices):
+    """Several microscaled matrices ((rows, cols, format) each, or None) in one
+    buffer, for what lives no longer than a call or is kept for one backward
+    pass: one allocation, and one tensor to keep. -> its size and the places."""
+    at, places = 0, []
+    for m in matrices:
+        if m is None:
+            places.append(None)
+            continue
+        rows, cols, format = m
+        scales = at + _up256(rows * _blocks(cols) * _CODE_BYTES[format])
+        places.append((at, scales, rows, cols, FORMATS[format]))
+        at = scales + _up256(_scale_bytes(rows, cols, format))
+    return at, tuple(places)
+
+
+def _placed(buffer, places):
+    """Descriptors of the matrices of a ``_layout`` in its buffer."""
+    base, index = buffer.data_ptr(), buffer.get_device()
+    return [None if p is None else _native.SbMx(base + p[0], base + p[1], p[2], p[3], p[4], index) for p in places]
+
+
+def _differentiable_once(backward):
+    """torch's once_differentiable, whose wrapping is only paid for where a
+    graph of the backward pass is asked for."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
+def _quantize_into(x, along, across):
+    x, rows, cols, stride = _matrix(x)
+    _check(_lib().sb_mx_quantize(x.data_ptr(), _DTYPES[x.dtype], rows, cols, stride, along, across,
+                                 _stream(x.get_device()), _scratch.ref))
+
+
+def _matmul_into(a, b, y):
+    _check(_lib().sb_mx_matmul(a, b, y.data_ptr(), _DTYPES[y.dtype], _stream(y.get_device()), _scratch.ref))
+    return y
 
 
 def quantize(x, format="mxfp4", *, along=-1):
@@ -236,15 +307,15 @@ def dequantize(q, dtype=torch.float16, *, transpose=False):
     rows, cols = q.shape
     out = torch.empty((cols, rows) if transpose else (rows, cols), dtype=dtype, device=q.device)
     if rows:
-        _check(_native.lib().sb_mx_dequantize(q.native, out.data_ptr(), _DTYPES[dtype], int(transpose),
-                                              _stream(q.device), _scratch.ref))
+        _check(_lib().sb_mx_dequantize(q.native, out.data_ptr(), _DTYPES[dtype], int(transpose),
+                                       _stream(q.get_device()), _scratch.ref))
     return out
 
 
 @lru_cache(maxsize=4096)
 def _linear_workspace(m, n, k, device):
     size = ctypes.c_int64()
-    _check(_native.lib().sb_mx_linear_workspace(m, n, k, device, ctypes.byref(size), _scratch.ref))
+    _check(_lib().sb_mx_linear_workspace(m, n, k, device, ctypes.byref(size), _scratch.ref))
     return size.value
 
 
@@ -259,23 +330,20 @@ def matmul(a, b, *, dtype=torch.bfloat16):
     if k != kb:
         raise ValueError(f"a [m, k] and b [n, k] need the same k: got {k} and {kb}")
     y = torch.empty((m, n), dtype=dtype, device=a.device)
-    if m and n:
-        _check(_native.lib().sb_mx_matmul(a.native, b.native, y.data_ptr(), _DTYPES[dtype], _stream(a.device),
-                                          _scratch.ref))
-    return y
+    return _matmul_into(a.native, b.native, y) if m and n else y
 
 
 def _linear(x, w, dtype):
-    lead = x.shape[:-1]
-    x, m, k, stride = _matrix(x, "x")
+    shape = x.shape
+    x, m, k, stride = _matrix(x)
     n = w.shape[0]
-    y = torch.empty((*lead, n), dtype=dtype, device=x.device)
+    y = x.new_empty((*shape[:-1], n), dtype=dtype)
     if m and n:
-        size = _linear_workspace(m, n, k, x.device.index)
-        space = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        _check(_native.lib().sb_mx_linear(x.data_ptr(), _DTYPES[x.dtype], m, stride, w.native, y.data_ptr(),
-                                          _DTYPES[dtype], space.data_ptr() if size else None, size,
-                                          _stream(x.device), _scratch.ref))
+        index = x.get_device()
+        size = _linear_workspace(m, n, k, index)
+        space = x.new_empty(size, dtype=torch.uint8) if size else None
+        _check(_lib().sb_mx_linear(x.data_ptr(), _DTYPES[x.dtype], m, stride, w.native, y.data_ptr(), _DTYPES[dtype],
+                                   space.data_ptr() if size else None, size, _stream(index), _scratch.ref))
     return y
 
 
@@ -289,7 +357,7 @@ class _FrozenLinear(torch.autograd.Function):
         return _linear(x, w, dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, dy):
         return _linear(dy, MxTensor(*ctx.saved_tensors, ctx.shape), ctx.dtype), None, None, None
 
@@ -301,28 +369,34 @@ class _TrainLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, dtype):
-        need_x, need_w = ctx.needs_input_grad[:2]
-        ctx.lead, ctx.dtypes = x.shape[:-1], (x.dtype, weight.dtype)
-        qx, qxt = _quantize(x, "mxfp4", True, need_w)
-        qw, qwt = _quantize(weight, "mxfp4", True, need_x)
-        kept = [q for q in (qxt, qwt) if q is not None]
-        ctx.shapes = [q.shape for q in kept]
-        ctx.save_for_backward(*(t for q in kept for t in (q.codes, q.scales)))
-        return matmul(qx, qw, dtype=dtype).view(*ctx.lead, weight.shape[0])
+        need_x, need_w, _ = ctx.needs_input_grad
+        n, k = weight.shape
+        m = x.numel() // k
+        ctx.dtypes, ctx.shape, ctx.extents = (x.dtype, weight.dtype), x.shape, (m, n, k)
+        size, places = _layout((m, k, "mxfp4"), (n, k, "mxfp4"))
+        now = x.new_empty(size, dtype=torch.uint8)
+        qx, qw = _placed(now, places)
+        size, ctx.places = _layout((k, m, "mxfp4") if need_w else None, (k, n, "mxfp4") if need_x else None)
+        kept = x.new_empty(size, dtype=torch.uint8)
+        qxt, qwt = _placed(kept, ctx.places)
+        ctx.save_for_backward(kept)
+        _quantize_into(x, qx, qxt)
+        _quantize_into(weight, qw, qwt)
+        return _matmul_into(qx, qw, x.new_empty((*x.shape[:-1], n), dtype=dtype))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, dy):
-        need_x, need_w = ctx.needs_input_grad[:2]
-        t = ctx.saved_tensors
-        kept = [MxTensor(t[2 * i], t[2 * i + 1], s) for i, s in enumerate(ctx.shapes)]
-        qdy, qdyt = _quantize(dy, "mxfp4", need_x, need_w)
-        dx = dw = None
-        if need_x:
-            dx = matmul(qdy, kept[-1], dtype=ctx.dtypes[0])
-            dx = dx.view(*ctx.lead, dx.shape[1])
-        if need_w:
-            dw = matmul(qdyt, kept[0], dtype=ctx.dtypes[1])
+        need_x, need_w, _ = ctx.needs_input_grad
+        m, n, k = ctx.extents
+        kept, = ctx.saved_tensors
+        qxt, qwt = _placed(kept, ctx.places)
+        size, places = _layout((m, n, "mxfp4") if need_x else None, (n, m, "mxfp4") if need_w else None)
+        now = dy.new_empty(size, dtype=torch.uint8)
+        qdy, qdyt = _placed(now, places)
+        _quantize_into(dy, qdy, qdyt)
+        dx = _matmul_into(qdy, qwt, dy.new_empty(ctx.shape, dtype=ctx.dtypes[0])) if need_x else None
+        dw = _matmul_into(qdyt, qxt, dy.new_empty((n, k), dtype=ctx.dtypes[1])) if need_w else None
         return dx, dw, None
 
 
@@ -340,20 +414,20 @@ def linear(x, weight, weight_t=None, *, dtype=None):
     axis that each product sums over, and the backward pass gives dx and dw."""
     _values(x, "x")
     dtype = _result(dtype, x.dtype)
-    if isinstance(weight, MxTensor):
+    if type(weight) is MxTensor:
         _mx(weight, "weight", "mxfp4")
     elif weight_t is not None:
         raise ValueError("weight_t goes with an MxTensor weight")
     elif _values(weight, "weight").dim() != 2:
         raise ValueError("weight is a matrix [n, k]")
-    if weight.device != x.device:
+    if weight.get_device() != x.get_device():
         raise ValueError("x and weight live on different devices")
     n, k = weight.shape
     if x.shape[-1] != k:
         raise ValueError(f"x [..., k] and weight [n, k] need the same k: got {x.shape[-1]} and {k}")
-    if isinstance(weight, MxTensor):
-        if not (torch.is_grad_enabled() and x.requires_grad):
-            return _linear(x.detach(), weight, dtype)
+    if type(weight) is MxTensor:
+        if not (x.requires_grad and torch.is_grad_enabled()):
+            return _linear(x, weight, dtype)
         if weight_t is None:
             raise ValueError("x needs a gradient: pass weight_t, the mxfp4 form of the weight's transpose")
         if _mx(weight_t, "weight_t", "mxfp4").shape != (k, n) or weight_t.device != x.device:
@@ -367,44 +441,42 @@ def linear(x, weight, weight_t=None, *, dtype=None):
 class _SiluMul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, up):
-        ctx.packed = up is None
-        ctx.shape = gate.shape
-        parts = gate.chunk(2, -1) if up is None else (gate, up)
-        h, kept = _silu_mul(*parts, True)
-        ctx.save_for_backward(*(t for q in kept for t in (q.codes, q.scales)))
-        ctx.extents = kept[0].shape
-        return h
+        ctx.packed, ctx.shape = up is None, gate.shape
+        if up is None:
+            gate, up = gate.chunk(2, -1)
+        cols = gate.shape[-1]
+        kept_matrix = (gate.numel() // cols, cols, "mxint8")
+        size, ctx.places = _layout(kept_matrix, kept_matrix)
+        kept = gate.new_empty(size, dtype=torch.uint8)
+        ctx.save_for_backward(kept)
+        return _silu_mul(gate, up, *_placed(kept, ctx.places))
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, dh):
-        t = ctx.saved_tensors
-        rows, cols = ctx.extents
-        dgate = torch.empty(ctx.shape, dtype=dh.dtype, device=dh.device)
-        dup = None if ctx.packed else torch.empty(ctx.shape, dtype=dh.dtype, device=dh.device)
-        if rows:
-            g, u = (MxTensor(t[i], t[i + 1], ctx.extents, "mxint8") for i in (0, 2))
-            dh, _, _, stride = _matrix(dh, "dh")
+        kept, = ctx.saved_tensors
+        gate, up = _placed(kept, ctx.places)
+        dgate = dh.new_empty(ctx.shape)
+        dup = None if ctx.packed else dh.new_empty(ctx.shape)
+        if gate.rows:
+            cols, dtype = gate.cols, dh.dtype
+            dh, _, _, stride = _matrix(dh)
             out = 2 * cols if ctx.packed else cols
             at = dgate.data_ptr() + cols * dh.element_size() if ctx.packed else dup.data_ptr()
-            _check(_native.lib().sb_silu_mul_backward(
-                dh.data_ptr(), stride, _DTYPES[dh.dtype], g.native, u.native, dgate.data_ptr(), out, at, out,
-                _stream(dh.device), _scratch.ref))
+            _check(_lib().sb_silu_mul_backward(dh.data_ptr(), stride, _DTYPES[dtype], gate, up, dgate.data_ptr(), out,
+                                               at, out, _stream(dh.get_device()), _scratch.ref))
         return dgate, dup
 
 
-def _silu_mul(gate, up, keep):
-    lead = gate.shape
-    gate, rows, cols, gate_stride = _matrix(gate, "gate")
-    up, _, _, up_stride = _matrix(up, "up")
-    h = torch.empty(lead, dtype=gate.dtype, device=gate.device)
-    kept = [MxTensor.empty(rows, cols, gate.device, "mxint8") for _ in range(2)] if keep else [None, None]
+def _silu_mul(gate, up, kept_gate=None, kept_up=None):
+    h = gate.new_empty(gate.shape)
+    gate, rows, cols, gate_stride = _matrix(gate)
+    up, _, _, up_stride = _matrix(up)
     if rows:
-        _check(_native.lib().sb_silu_mul(
-            gate.data_ptr(), gate_stride, up.data_ptr(), up_stride, _DTYPES[gate.dtype], rows, cols,
-            gate.device.index, h.data_ptr(), kept[0].native if keep else None, kept[1].native if keep else None,
-            _stream(gate.device), _scratch.ref))
-    return h, kept
+        index = gate.get_device()
+        _check(_lib().sb_silu_mul(gate.data_ptr(), gate_stride, up.data_ptr(), up_stride, _DTYPES[gate.dtype], rows,
+                                  cols, index, h.data_ptr(), kept_gate, kept_up, _stream(index), _scratch.ref))
+    return h
 
 
 def silu_mul(gate, up=None):
@@ -425,5 +497,4 @@ def silu_mul(gate, up=None):
             raise ValueError("gate and up have the same shape, type and device")
     if torch.is_grad_enabled() and (gate.requires_grad or (up is not None and up.requires_grad)):
         return _SiluMul.apply(gate, up)
-    parts = gate.detach().chunk(2, -1) if up is None else (gate.detach(), up.detach())
-    return _silu_mul(*parts, False)[0]
+    return _silu_mul(*(gate.detach().chunk(2, -1) if up is None else (gate.detach(), up.detach())))
