@@ -146,8 +146,8 @@ uint64_t sbc_wait_launch_count(void);
 void sbc_set_wait_limit_ns(uint64_t ns);
 
 /* ---- test hooks (never armed by the library itself) ---------------------
- * Failure injection for the tests of the error paths; neither hook faults,
- * traps or hangs a GPU.
+ * Failure injection for the tests of the error paths; no hook faults, traps
+ * or hangs a GPU.
  *
  * sbc_test_fault_mode: make this layer's CUDA calls report cudaErrorUnknown
  * on the host without issuing them (the work already queued still runs):
@@ -164,6 +164,11 @@ void sbc_set_wait_limit_ns(uint64_t ns);
  * tile run out of their bounded wait after `wait_limit_ns` (0: the current
  * limit), set the descriptor's fault word and leave; the launch after it is
  * normal again. job = UINT32_MAX disarms. */
+/* sbc_test_withhold_mx: the next mxfp4 product (any device) issues no copy of
+ * the weight codes of its first step, so its waits run out after
+ * `wait_limit_ns`, sbc_mx_take_fault reports it, and the launch after it is
+ * normal again. 0 disarms. */
+void sbc_test_withhold_mx(uint64_t wait_limit_ns);
 int sbc_test_fault_mode(int mode);
 void sbc_test_withhold_tile(uint32_t job, uint64_t wait_limit_ns);
 

@@ -137,7 +137,8 @@ _cuda = None
 def cuda_layer():
     """The thin CUDA layer (libsb_cuda.so, include/sb_cuda.h), loaded by the
     runtime library; for its wait-limit setting and the test hooks that
-    inject failures (``sbc_test_fault_mode``, ``sbc_test_withhold_tile``)."""
+    inject failures (``sbc_test_fault_mode``, ``sbc_test_withhold_tile``,
+    ``sbc_test_withhold_mx``)."""
     global _cuda
     if _cuda is not None:
         return _cuda
@@ -147,6 +148,8 @@ def cuda_layer():
     L.sbc_test_fault_mode.argtypes = [ctypes.c_int]
     L.sbc_test_withhold_tile.restype = None
     L.sbc_test_withhold_tile.argtypes = [ctypes.c_uint32, ctypes.c_uint64]
+    L.sbc_test_withhold_mx.restype = None
+    L.sbc_test_withhold_mx.argtypes = [ctypes.c_uint64]
     L.sbc_set_wait_limit_ns.restype = None
     L.sbc_set_wait_limit_ns.argtypes = [ctypes.c_uint64]
     L.sbc_wait_launch_count.restype = ctypes.c_uint64

@@ -54,6 +54,7 @@ struct ProductArgs {
   int32_t x_vec;    // FUSED: rows of x start on 16-byte boundaries
   int32_t y_vec;    // N is a multiple of 4 and y starts on a 16-byte boundary
   int32_t after_quantize; // launched to overlap the end of the kernel that writes A and its scales
+  int32_t withhold;       // test hook: the first CTA issues no copy of B's codes for its first step
 };
 
 // Two CTAs fit an SM (228 KB): 100 to 113 KB of stages, and at most 256 of the
@@ -73,7 +74,7 @@ template <int NT, bool FUSED> struct Shape {
   static constexpr int kStepA = FUSED ? NT * 128 : 0;
   static constexpr int kScaleA = FUSED ? 2 * kTileA : 0;
   static constexpr int kAcc = NT < 32 ? 32 : NT;                    // columns of the accumulator
-  static constexpr int kCols = kAcc + 32 <= 64 ? 64 : kAcc + 32 <= 128 ? 128 : 256; // + two buffers of 8 + 8 scale columns
+  static constexpr int kCols = kAcc + 64 <= 128 ? 128 : 256;        // + four buffers of 8 + 8 scale columns
 };
 
 // The loading and the multiplying warp run their loops as a whole, and one
@@ -223,7 +224,8 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
     const auto load_b = [&](uint32_t ks, int st) {
       const uint32_t at = stage0 + st * S::kStage, bar = smem_addr(&full[st]);
       expect_bytes(bar, S::kBytesB + S::kBytesA + (FUSED ? 1 : 2) * scale_bytes(ks));
-      load_box(at, &a.map_b, ks * 128, tb * kRowsB, bar);
+      if (!(a.withhold && blockIdx.x == 0 && ks == ks0))
+        load_box(at, &a.map_b, ks * 128, tb * kRowsB, bar);
       load_bytes(at + S::kScales, sb + static_cast<int64_t>(ks) * 1024, scale_bytes(ks), bar);
     };
     const auto load_a = [&](uint32_t ks, int st) {
@@ -262,7 +264,9 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
       warp_wait(&full[i], i < st ? phase ^ 1 : phase, a.wait_ns);
   } else if (warp == 1) {
     // Scales go to tensor memory one stage ahead of the products that use
-    // them (two buffers of columns), so that no product waits for its own.
+    // them, so that no product waits for its own; four buffers of columns, so
+    // that a copy lies three stages of products behind the last that read its
+    // columns.
     int st = 0, next = 0;
     uint32_t phase = 0;
     const auto scales = [&](uint32_t ks) {
@@ -272,7 +276,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
       const uint32_t at = stage0 + next * S::kStage + S::kScales;
       const uint32_t at_sa =
           FUSED ? own_a + (ks1 - ks0) * S::kStepA + (ks - ks0) * S::kScaleA : at + kScaleStage;
-      const uint32_t sb = tmem + S::kAcc + (ks & 1) * 16, sa = sb + 8;
+      const uint32_t sb = tmem + S::kAcc + (ks & 3) * 16, sa = sb + 8;
       const uint32_t tiles = a.quads - 2 * ks < 2 ? 1 : 2;
       for (uint32_t q = 0; q < tiles; ++q) {
         copy_scales(sb + 4 * q, at + q * 512);
@@ -291,7 +295,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
       const uint32_t left = a.k64 - 4 * ks, mmas = left < 4 ? left : 4;
       const uint32_t at = stage0 + st * S::kStage;
       const uint32_t at_a = FUSED ? own_a + (ks - ks0) * S::kStepA : at + S::kBytesB;
-      const uint32_t sb = tmem + S::kAcc + (ks & 1) * 16, sa = sb + 8;
+      const uint32_t sb = tmem + S::kAcc + (ks & 3) * 16, sa = sb + 8;
       const uint64_t desc_b = codes_desc(at), desc_a = codes_desc(at_a); // 32 bytes on: + 2
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i)
@@ -451,6 +455,7 @@ struct PairArgs {
   uint32_t tiles_a, tiles_b;
   int32_t y_vec; // N is a multiple of 8 and y starts on a 16-byte boundary
   int32_t after_quantize;
+  int32_t withhold; // test hook, as in ProductArgs
 };
 
 template <int NB> struct PairShape {
@@ -578,7 +583,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_mx_product_pair(const __gri
         if (rank == 0)
           expect_bytes(smem_addr(&full[st]), 2 * S::kStage);
         const uint32_t at = stage0 + st * S::kStage, bar = first_full + 8 * st;
-        load_box_pair(at, &a.map_b, ks * 128, row_b, bar);
+        if (!(a.withhold && blockIdx.x == 0 && armed == 0))
+          load_box_pair(at, &a.map_b, ks * 128, row_b, bar);
         load_box_pair(at + S::kBytesB, &a.map_a, ks * 128, row_a, bar);
         load_box_pair(at + S::kScales, &a.map_scales_b, 0, scale_b + 2 * ks, bar);
 #pragma unroll
@@ -600,16 +606,16 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_mx_product_pair(const __gri
   } else if (warp == 1 && rank == 0) {
     constexpr uint32_t kInstr = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(NB / 8) << 17) | (1u << 23) | (2u << 27);
     // Scales go to tensor memory one stage ahead of the products that use
-    // them (two buffers of columns), so that no product waits for its own.
+    // them; four buffers of columns (see k_mx_product).
     int st = 0, next = 0;
-    uint32_t phase = 0, turn = 0;
+    uint32_t phase = 0, turn = 0, copied = 0, used = 0;
     bool ok = true;
     const auto scales = [&](uint32_t ks) {
       if (!warp_wait(&full[next], phase, a.wait_ns))
         return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t at = stage0 + next * S::kStage + S::kScales;
-      const uint32_t sb = tmem + S::kScaleCol + (ks & 1) * 32, sa = sb + 8;
+      const uint32_t sb = tmem + S::kScaleCol + (copied++ & 3) * 32, sa = sb + 8;
       const uint32_t tiles = a.quads - 2 * ks < 2 ? 1 : 2;
       for (uint32_t q = 0; q < tiles; ++q) {
         copy_scales_pair(sb + 4 * q, at + q * 512);
@@ -638,7 +644,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_mx_product_pair(const __gri
           ok = scales(ks + 1);
         const uint32_t left = a.k64 - 4 * ks, mmas = left < 4 ? left : 4;
         const uint32_t at = stage0 + st * S::kStage;
-        const uint32_t sb = tmem + S::kScaleCol + (ks & 1) * 32, sa = sb + 8;
+        const uint32_t sb = tmem + S::kScaleCol + (used++ & 3) * 32, sa = sb + 8;
         const uint64_t desc_b = codes_desc(at), desc_a = codes_desc(at + S::kBytesB); // 32 bytes on: + 2
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j)
@@ -684,13 +690,29 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_mx_product_pair(const __gri
         // stored transposed by stmatrix: [column][32 rows] in shared memory,
         // 64 bytes per column, 16-byte pieces swapped so that eight columns
         // cover all banks. From there each lane stores 16 bytes of a row of y.
-        uint32_t v[NB / 64][2][16];
+        uint32_t p[NB / 64][2][8];
 #pragma unroll
-        for (int c = 0; c < NB / 64; ++c)
+        for (int round = 0; round < 2; ++round) { // half the columns at a time bounds the registers
+          constexpr int kC = (NB / 64 + 1) / 2, kAll = NB / 64;
+          uint32_t v[kC][2][16];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            read16x32(v[c][h], acc + (static_cast<uint32_t>(h * 16) << 16) + c * 32);
-        release();
+          for (int c = 0; c < kC; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (round * kC + c < kAll)
+                read16x32(v[c][h], acc + (static_cast<uint32_t>(h * 16) << 16) + (round * kC + c) * 32);
+          if (round == 0)
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          else
+            release();
+#pragma unroll
+          for (int c = 0; c < kC && round * kC + c < kAll; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                p[round * kC + c][h][k] = pack2<DT>(__uint_as_float(v[c][h][2 * k]), __uint_as_float(v[c][h][2 * k + 1]));
+        }
         const uint32_t turn_at = stage0 + S::kStages * S::kStage + (warp - 4) * 2048;
 #pragma unroll
         for (int c = 0; c < NB / 64; ++c) {
@@ -703,11 +725,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_mx_product_pair(const __gri
             for (int g = 0; g < 2; ++g) { // 16 columns: matrices (rows 0-7, 8-15) x (columns 0-7, 8-15)
               const int col = g * 16 + (lane >> 4) * 8 + (lane & 7), piece = h * 2 + (lane >> 3 & 1);
               const uint32_t at = turn_at + col * 64 + ((piece ^ (col >> 1 & 3)) << 4);
-              const auto pair = [&](int k) {
-                return pack2<DT>(__uint_as_float(v[c][h][8 * g + 2 * k]), __uint_as_float(v[c][h][8 * g + 2 * k + 1]));
-              };
               asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at),
-                           "r"(pair(0)), "r"(pair(1)), "r"(pair(2)), "r"(pair(3))
+                           "r"(p[c][h][4 * g]), "r"(p[c][h][4 * g + 1]), "r"(p[c][h][4 * g + 2]),
+                           "r"(p[c][h][4 * g + 3])
                            : "memory");
             }
           __syncwarp();
@@ -796,19 +816,22 @@ struct Plan {
 /// x [11008, 4096] 9.5 against 10.7 us in two launches; with 12 row steps 10.6
 /// against 10.7, with 24 12.6 against 10.8.
 ///
-/// More rows: every kernel is then bound by what the SMs take from L2, about
-/// 45 bytes per cycle each, so the cost of a step goes with its bytes and the
-/// cost of a launch with the rounds of tiles that the SMs need. The cycles
-/// below (per step, per tile) are fits to measured times: 2048 x 11008 x 4096
-/// with 256, 192, 128 rows of A a pair and single CTAs 49, 52, 62, 88 us; 512 x
-/// 11008 x 4096 21.8, 18.8, 21.5, 33.1; 256 x 4096 x 4096 13.2, 12.1, 11.2,
-/// 12.4; 256 x 1024 x 8192 18.3, 16.4, 18.2, 12.4.
+/// More rows: pairs of SMs with 256, 192 or 128 rows of A a tile, or the tiles of
+/// one CTA with their split. The cost of each is the rounds of tiles that the
+/// SMs need times a tile's cycles, which are fits to measured times (steps of
+/// 700, 600, 520 and 700 cycles, and what a tile costs beside them); over 36
+/// shapes the choice by them loses 0.2 % against the best of the four. Measured,
+/// us, pairs of 256 / 192 / 128 / single CTAs: 2048 x 11008 x 4096 43.7 / 47.6 /
+/// 58.6 / 82.7; 512 x 11008 x 4096 21.9 / 20.7 / 22.8 / 32.7; 256 x 4096 x 4096
+/// 13.0 / 11.9 / 11.3 / 12.2; 256 x 1024 x 8192 23.4 / 21.5 / 17.9 / 12.6.
 bool plan_of(int64_t m, int64_t n, int64_t k, int sms, Plan *p) {
   p->nt = m <= 8 ? 8 : m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
   p->tiles_a = (m + p->nt - 1) / p->nt;
   p->tiles_b = (n + kRowsB - 1) / kRowsB;
   p->steps = (k + kStep - 1) / kStep;
-  if (sms <= 1 || p->steps > INT32_MAX / 8 || p->tiles_a > INT32_MAX / 8 / p->tiles_b)
+  // coordinates of the copies (rows, bytes along K) are 31-bit
+  if (sms <= 1 || m > INT32_MAX - 256 || n > INT32_MAX - 256 || k > INT32_MAX || p->tiles_a > INT32_MAX / 8 / p->tiles_b ||
+      (m > n ? m : n) / 128 + 2 > INT32_MAX / quads_of(k))
     return false;
   const int64_t tiles = p->tiles_a * p->tiles_b;
   int64_t split = sms / tiles;
@@ -824,8 +847,8 @@ bool plan_of(int64_t m, int64_t n, int64_t k, int sms, Plan *p) {
   p->pair = 0;
   if (m > 128) {
     const double ctas = static_cast<double>(tiles * p->split) / sms;
-    double best = (ctas < 1 ? 1 : ctas) * each * 774 + 4000;
-    const struct { int rows, step, tile; } pairs[] = {{256, 796, 1800}, {192, 700, 1000}, {128, 590, 1000}};
+    double best = (ctas < 1 ? 1 : ctas) * each * 700 + 6000;
+    const struct { int rows, step, tile; } pairs[] = {{256, 700, 2500}, {192, 600, 2500}, {128, 520, 2000}};
     for (const auto &c : pairs) {
       const int64_t t = (m + c.rows - 1) / c.rows * ((n + 255) / 256), rounds = (t + sms / 2 - 1) / (sms / 2);
       const double cost = static_cast<double>(rounds) * (p->steps * c.step + c.tile);
@@ -917,6 +940,7 @@ template <int DT, int NB> int launch_pair(const ProductArgs &a, const sbc_mx *qa
   args.tiles_b = static_cast<uint32_t>((a.n + 255) / 256);
   args.y_vec = a.n % 8 == 0 && reinterpret_cast<uintptr_t>(a.y) % 16 == 0;
   args.after_quantize = a.after_quantize;
+  args.withhold = a.withhold;
   auto k = k_mx_product_pair<DT, NB>;
   cudaError_t e = allow_shared<k_mx_product_pair<DT, NB>>();
   if (e != cudaSuccess)
@@ -970,6 +994,9 @@ int launch_plan(const ProductArgs &a, const Plan &p, const sbc_mx *qa, const sbc
   }
 }
 
+/// Armed by sbc_test_withhold_mx: the wait limit of the next launch.
+std::atomic<uint64_t> g_withhold{0};
+
 /// The word in mapped pinned host memory that kernels set to 2 when a wait
 /// runs out: one for the process, allocated on first use.
 int32_t *fault_word() {
@@ -992,6 +1019,8 @@ int32_t *fault_word() {
 } // namespace
 
 extern "C" {
+
+void sbc_test_withhold_mx(uint64_t wait_limit_ns) { g_withhold.store(wait_limit_ns, std::memory_order_relaxed); }
 
 int sbc_mx_take_fault(void) {
   int32_t *w = fault_word();
@@ -1027,6 +1056,10 @@ int sbc_mx_product(const sbc_mx *a, const void *x, int32_t x_dtype, int64_t x_st
   args.y_vec = b->rows % 4 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
   args.fault = fault;
   args.wait_ns = wait_limit_ns();
+  if (const uint64_t limit = g_withhold.exchange(0, std::memory_order_relaxed)) {
+    args.withhold = 1;
+    args.wait_ns = limit;
+  }
   args.m = a->rows;
   args.n = b->rows;
   args.k = a->cols;

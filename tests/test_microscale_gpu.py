@@ -173,6 +173,49 @@ def test_linear(m, n, k, name):
     assert torch.equal(y, mx.matmul(mx.quantize(x), qw, dtype=t))
 
 
+# pairs of SMs with 256, 192 and 128 rows a tile (one round of tiles and more,
+# widths that 16-byte stores fit and do not), and single CTAs with a split
+MANY_ROWS = [(1003, 4101, 520), (2000, 4104, 64), (1500, 5000, 96), (700, 8200, 130), (300, 9001, 520), (129, 129, 33),
+             (520, 1100, 2080), (300, 300, 257), (180, 300, 4000), (257, 1000, 3000), (1100, 10000, 70)]
+
+
+@pytest.mark.parametrize("m,n,k", MANY_ROWS)
+def test_many_rows(m, n, k):
+    x, w = tensor((m, k), torch.bfloat16, 50), mx.quantize(tensor((n, k), torch.float32, 51, std=0.02))
+    a, b = O.rounded(host(x)), O.rounded(host(tensor((n, k), torch.float32, 51, std=0.02)))
+    for t in (torch.float16, torch.float32):
+        y = mx.linear(x, w, dtype=t)
+        assert torch.equal(y, mx.linear(x, w, dtype=t))
+        check_product(y, a, b)
+
+
+def test_result_rows_do_not_depend_on_their_company():
+    """Rows of a batch that a kernel takes whole (no split along K) are those of
+    the same rows in a larger one."""
+    x, w = tensor((512, 256), torch.bfloat16, 52), mx.quantize(tensor((384, 256), torch.float32, 53))
+    y = mx.linear(x, w)
+    for m in (1, 7, 16, 33, 128, 129, 300):
+        assert torch.equal(mx.linear(x[:m], w), y[:m])
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 512, 2048), (40, 1000, 4096), (700, 8200, 512)])
+def test_wait_that_runs_out_is_reported_by_the_next_product(m, n, k):
+    """A withheld copy: the kernel's bounded waits run out, it leaves by itself,
+    the next product reports it and the one after is right again."""
+    from sym_b200 import _native, pyreloc
+
+    x, w = tensor((m, k), torch.float16, 54), mx.quantize(tensor((n, k), torch.float32, 55))
+    want = mx.linear(x, w)
+    torch.cuda.synchronize()
+    _native.cuda_layer().sbc_test_withhold_mx(20_000_000)
+    mx.linear(x, w)
+    torch.cuda.synchronize()
+    with pytest.raises(pyreloc.TransferError) as e:
+        mx.linear(x, w)
+    assert e.value.code == "backend_failure"
+    assert torch.equal(mx.linear(x, w), want)
+
+
 def test_linear_leading_axes_and_result_type():
     w = mx.quantize(tensor((96, 64), torch.bfloat16, 5))
     x = tensor((2, 3, 64), torch.bfloat16, 6)
