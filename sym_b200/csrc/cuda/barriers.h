@@ -17,16 +17,16 @@ void count_launch();
 void count_wait_launch();
 uint64_t wait_limit_ns();
 
-/// Lets a kernel use all the dynamic shared memory a block may have (226 KB
-/// beside its static variables) on the current device; the driver is asked
-/// once per kernel and device.
-template <auto KERNEL> cudaError_t allow_shared() {
+/// Lets a kernel use `bytes` of dynamic shared memory (the same number in every
+/// call for a kernel) on the current device; the driver is asked once per
+/// kernel and device.
+template <auto KERNEL> cudaError_t allow_shared(int bytes) {
   static std::atomic<bool> allowed[64];
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess || (device < 64 && allowed[device].load(std::memory_order_relaxed)))
     return e;
-  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess && device < 64)
     allowed[device].store(true, std::memory_order_relaxed);
   return e;

@@ -93,6 +93,38 @@ template <int DT> struct Place {
   }
 };
 
+/// One matrix's parts of a thread block's rows, and their stores, when rows have
+/// no alignment.
+template <int DT> struct RaggedRows {
+  using U = Bits<DT>;
+  using R = Ragged<U, Part<DT>::kValues>;
+  static constexpr int kStride = Place<DT>::kStride;
+  int64_t r, c0;
+  int n;
+  uint8_t *scratch;
+  __device__ __forceinline__ RaggedRows(const GateArgs &a, uint4 (*shared)[kScratch / 16]) {
+    r = (static_cast<int64_t>(blockIdx.z) * kMaxY + blockIdx.y) * kRows + (threadIdx.x >> 5) * R::kRows;
+    c0 = static_cast<int64_t>(blockIdx.x) * kTile;
+    const int64_t left = a.cols - c0;
+    n = static_cast<int>(left < kTile ? left : kTile);
+    scratch = reinterpret_cast<uint8_t *>(shared[threadIdx.x >> 5]);
+  }
+  __device__ __forceinline__ int rows(const GateArgs &a, int unit) const {
+    const int64_t there = a.rows - r - unit * kStride;
+    return static_cast<int>(there < R::kRows ? there : R::kRows);
+  }
+  __device__ __forceinline__ void fetch(R &ragged, const GateArgs &a, const void *x, int64_t stride, int unit) const {
+    ragged.fetch(static_cast<const U *>(x) + (r + unit * kStride) * stride + c0, stride, rows(a, unit), n);
+  }
+  __device__ __forceinline__ void store(const GateArgs &a, void *x, int64_t stride, int unit,
+                                        const float2 (&v)[Part<DT>::kValues / 8][4]) const {
+    uint4 words[2];
+    to_words<DT, Part<DT>::kValues / 8>(words, v);
+    ragged_store<U, Part<DT>::kValues>(words, scratch, static_cast<U *>(x) + (r + unit * kStride) * stride + c0, stride,
+                                       rows(a, unit), n);
+  }
+};
+
 template <int DT, bool KEEP, bool VEC>
 __global__ void __launch_bounds__(kThreads, 3) k_silu_mul(const __grid_constant__ GateArgs a) {
   using T = typename Value<DT>::T;
@@ -104,11 +136,27 @@ __global__ void __launch_bounds__(kThreads, 3) k_silu_mul(const __grid_constant_
   T *h_at = static_cast<T *>(a.h) + p.r0 * a.cols + p.c;
   const int64_t block = p.r0 * a.blocks + p.c / kBlock;
   Part<DT> gate[P::kUnits], up[P::kUnits];
+  __shared__ uint4 scratch[VEC ? 1 : kThreads / 32][kScratch / 16];
+  const RaggedRows<DT> ragged(a, scratch);
+  if constexpr (VEC) {
 #pragma unroll
-  for (int i = 0; i < P::kUnits; ++i) {
-    const int have = p.r0 + P::kStride * i < a.rows ? p.cols : 0;
-    gate[i].template load<VEC>(gate_at + P::kStride * i * a.gate_stride, have);
-    up[i].template load<VEC>(up_at + P::kStride * i * a.up_stride, have);
+    for (int i = 0; i < P::kUnits; ++i) {
+      const int have = p.r0 + P::kStride * i < a.rows ? p.cols : 0;
+      gate[i].template load<true>(gate_at + P::kStride * i * a.gate_stride, have);
+      up[i].template load<true>(up_at + P::kStride * i * a.up_stride, have);
+    }
+  } else {
+    typename RaggedRows<DT>::R in[P::kUnits][2];
+#pragma unroll
+    for (int i = 0; i < P::kUnits; ++i) {
+      ragged.fetch(in[i][0], a, a.gate, a.gate_stride, i);
+      ragged.fetch(in[i][1], a, a.up, a.up_stride, i);
+    }
+#pragma unroll
+    for (int i = 0; i < P::kUnits; ++i) {
+      in[i][0].place(reinterpret_cast<uint4 *>(&gate[i]), ragged.scratch);
+      in[i][1].place(reinterpret_cast<uint4 *>(&up[i]), ragged.scratch);
+    }
   }
 #pragma unroll
   for (int i = 0; i < P::kUnits; ++i) {
@@ -123,8 +171,10 @@ __global__ void __launch_bounds__(kThreads, 3) k_silu_mul(const __grid_constant_
         h[j][k] = __fmul2_rn(__fmul2_rn(g[k], sigmoid2<DT>(g[k])), u[k]);
     }
     const bool row_exists = p.r0 + P::kStride * i < a.rows;
-    if (row_exists)
-      store_part<DT, VEC>(h_at + P::kStride * i * a.cols, h, p.cols);
+    if constexpr (!VEC)
+      ragged.store(a, a.h, a.cols, i, h);
+    else if (row_exists)
+      store_part<DT, true>(h_at + P::kStride * i * a.cols, h, p.cols);
     if (KEEP) {
       const bool exists = row_exists && p.c < a.blocks * kBlock;
       const int64_t at = block + P::kStride * i * a.blocks;
@@ -140,8 +190,11 @@ __global__ void __launch_bounds__(kThreads) k_silu_mul_backward(const __grid_con
   using P = Place<DT>;
   constexpr int N = Part<DT>::kValues / 8;
   const P p(a);
-  if (p.cols <= 0)
+  if (VEC && p.cols <= 0)
     return;
+  __shared__ uint4 scratch[VEC ? 1 : kThreads / 32][kScratch / 16];
+  const RaggedRows<DT> ragged(a, scratch);
+  typename RaggedRows<DT>::R elements[VEC ? 1 : P::kUnits];
   Part<DT> in[P::kUnits];
   uint2 gate[P::kUnits][N], up[P::kUnits][N];
   uint32_t gate_scale[P::kUnits], up_scale[P::kUnits];
@@ -158,9 +211,12 @@ __global__ void __launch_bounds__(kThreads) k_silu_mul_backward(const __grid_con
   };
 #pragma unroll
   for (int i = 0; i < P::kUnits; ++i) {
-    if (p.r0 + P::kStride * i < a.rows) {
+    if constexpr (!VEC)
+      ragged.fetch(elements[i], a, a.gate, a.gate_stride, i);
+    if (p.r0 + P::kStride * i < a.rows && (VEC || p.c < a.blocks * kBlock)) {
       const int64_t block = block0 + P::kStride * i * a.blocks;
-      in[i].template load<VEC>(dh_at + P::kStride * i * a.gate_stride, p.cols);
+      if constexpr (VEC)
+        in[i].template load<true>(dh_at + P::kStride * i * a.gate_stride, p.cols);
       codes(gate[i], a.gate_codes + block * 32 + p.in_block);
       codes(up[i], a.up_codes + block * 32 + p.in_block);
       gate_scale[i] = __ldg(a.gate_scales + block);
@@ -171,8 +227,10 @@ __global__ void __launch_bounds__(kThreads) k_silu_mul_backward(const __grid_con
   T *dup_at = static_cast<T *>(a.dup) + p.r0 * a.dup_stride + p.c;
 #pragma unroll
   for (int i = 0; i < P::kUnits; ++i) {
-    if (p.r0 + P::kStride * i >= a.rows)
+    if (VEC && p.r0 + P::kStride * i >= a.rows)
       return;
+    if constexpr (!VEC)
+      elements[i].place(reinterpret_cast<uint4 *>(&in[i]), ragged.scratch);
     const float gs = scale_value<SBC_MXINT8>(gate_scale[i]), us = scale_value<SBC_MXINT8>(up_scale[i]);
     const float2 one = make_float2(1.f, 1.f);
     float2 dg[N][4], du[N][4];
@@ -190,8 +248,13 @@ __global__ void __launch_bounds__(kThreads) k_silu_mul_backward(const __grid_con
         du[j][k] = __fmul2_rn(dh[k], __fmul2_rn(g[k], s));
       }
     }
-    store_part<DT, VEC>(dgate_at + P::kStride * i * a.h_stride, dg, p.cols);
-    store_part<DT, VEC>(dup_at + P::kStride * i * a.dup_stride, du, p.cols);
+    if constexpr (VEC) {
+      store_part<DT, true>(dgate_at + P::kStride * i * a.h_stride, dg, p.cols);
+      store_part<DT, true>(dup_at + P::kStride * i * a.dup_stride, du, p.cols);
+    } else {
+      ragged.store(a, a.h, a.h_stride, i, dg);
+      ragged.store(a, a.dup, a.dup_stride, i, du);
+    }
   }
 }
 

@@ -881,7 +881,7 @@ template <int DT, int XT, int NT, bool FUSED> int launch(const ProductArgs &a, c
   auto k = k_mx_product<DT, XT, NT, FUSED>;
   const int own = FUSED ? static_cast<int>((p.steps + p.split - 1) / p.split) * (S::kStepA + S::kScaleA) + 512 : 0;
   const int bytes = S::kStages * S::kStage + own + 1024; // + the alignment of the first stage
-  cudaError_t e = allow_shared<k_mx_product<DT, XT, NT, FUSED>>();
+  cudaError_t e = allow_shared<k_mx_product<DT, XT, NT, FUSED>>(kSmemMax - 1024);
   if (e != cudaSuccess)
     return e;
   cudaLaunchAttribute attr[2]{};
@@ -942,7 +942,7 @@ template <int DT, int NB> int launch_pair(const ProductArgs &a, const sbc_mx *qa
   args.after_quantize = a.after_quantize;
   args.withhold = a.withhold;
   auto k = k_mx_product_pair<DT, NB>;
-  cudaError_t e = allow_shared<k_mx_product_pair<DT, NB>>();
+  cudaError_t e = allow_shared<k_mx_product_pair<DT, NB>>(PairShape<NB>::kSmem);
   if (e != cudaSuccess)
     return e;
   const uint32_t tiles = args.tiles_a * args.tiles_b, pairs = static_cast<uint32_t>(sms / 2);

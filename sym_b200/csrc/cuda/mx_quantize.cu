@@ -60,6 +60,27 @@ __device__ __forceinline__ void quantize_part(const Raw8<DT> (&in)[V / 8], float
     *scales = static_cast<uint8_t>(exists ? byte : 0);
 }
 
+/// The parts of a block's rows from r0 on, whose starts have no alignment.
+template <int DT, int UNITS>
+__device__ __forceinline__ void load_ragged(Part<DT> (&in)[UNITS], const QuantizeArgs &a, int64_t r0, int64_t c0) {
+  __shared__ uint4 scratch[kThreads / 32][kScratch / 16];
+  using R = Ragged<Bits<DT>, Part<DT>::kValues>;
+  constexpr int kStride = kThreads / Part<DT>::kLanes;
+  const int warp = threadIdx.x >> 5;
+  const int64_t r = r0 + warp * R::kRows, left = a.cols - c0;
+  const Bits<DT> *x = static_cast<const Bits<DT> *>(a.x) + r * a.row_stride + c0;
+  R ragged[UNITS];
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const int64_t rows = a.rows - r - i * kStride;
+    ragged[i].fetch(x + i * kStride * a.row_stride, a.row_stride, rows < R::kRows ? static_cast<int>(rows) : R::kRows,
+                    left < kTile ? static_cast<int>(left) : kTile);
+  }
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i)
+    ragged[i].place(reinterpret_cast<uint4 *>(&in[i]), reinterpret_cast<uint8_t *>(scratch[warp]));
+}
+
 /// Blocks along the columns only: 64 rows (FEW: as many as one unit a thread
 /// covers) x 128 columns per block of threads, the loads of all units before
 /// the first use.
@@ -79,9 +100,13 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize(const __grid_constant_
   const T *x = static_cast<const T *>(a.x) + r0 * a.row_stride + c;
   const int rows = static_cast<int>(a.rows - r0 < 64 ? a.rows - r0 : 64); // from r0 on
   Part<DT> in[kUnits];
+  if constexpr (VEC) {
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i)
-    in[i].template load<VEC>(x + i * kStride * a.row_stride, i * kStride < rows ? have : 0);
+    for (int i = 0; i < kUnits; ++i)
+      in[i].template load<true>(x + i * kStride * a.row_stride, i * kStride < rows ? have : 0);
+  } else {
+    load_ragged<DT, kUnits>(in, a, static_cast<int64_t>(tr) * (kUnits * kStride), static_cast<int64_t>(tc) * kTile);
+  }
   const int64_t blocks = blocks_of(a.cols);
   const bool exists = c < blocks * kBlock;
   constexpr int kBytes = FMT == SBC_MXFP4 ? 16 : 32; // of codes per block
@@ -121,9 +146,13 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize_across(const __grid_co
   uint8_t *row_codes = a.codes + (r0 + row0) * row_blocks * 16 + c / 2;
   uint8_t *row_scales = a.scales + scale_word(r0 + row0, tc, quads_of(a.cols)) + c8 / 32;
   Part<DT> in[kUnits];
+  if constexpr (VEC) {
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i)
-    in[i].template load<VEC>(x + i * kStride * a.row_stride, row0 + i * kStride < here ? have : 0);
+    for (int i = 0; i < kUnits; ++i)
+      in[i].template load<true>(x + i * kStride * a.row_stride, row0 + i * kStride < here ? have : 0);
+  } else {
+    load_ragged<DT, kUnits>(in, a, r0, c0);
+  }
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
     const int row = row0 + i * kStride;
@@ -218,9 +247,10 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const __grid_constan
   const int64_t c = static_cast<int64_t>(tc) * kTile + c8, left = a.cols - c;
   const int have = static_cast<int>(left < V ? left : V);
   const int rows = static_cast<int>(a.rows - r0 < 64 ? a.rows - r0 : 64); // from r0 on
-  if (have <= 0 || rows <= 0)
+  if (VEC && (have <= 0 || rows <= 0))
     return;
   const int64_t blocks = blocks_of(a.cols);
+  const bool exists = c < blocks * kBlock;
   // four 4-bit codes are half a word, which two lanes read
   const uint8_t *codes_at = a.codes + r0 * blocks * kBytes + (c * kBytes / 32 & ~int64_t{3});
   const bool upper = V * kBytes / 32 == 2 && (c & 4);
@@ -229,7 +259,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const __grid_constan
   uint32_t scale[kUnits];
 #pragma unroll
   for (int i = 0; i < kUnits; ++i)
-    if (i * kStride < rows) {
+    if (i * kStride < rows && (VEC || exists)) {
       const int64_t step = FMT == SBC_MXFP4 ? (i * kStride / 32) * 4 + (i * kStride % 32) * 16 : i * kStride * blocks;
       codes[i] = __ldg(reinterpret_cast<const C *>(codes_at + i * (kStride * kBytes) * blocks));
       scale[i] = __ldg(scales + step);
@@ -237,7 +267,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const __grid_constan
   T *out = static_cast<T *>(a.out) + r0 * a.cols + c;
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
-    if (i * kStride >= rows)
+    if (VEC && i * kStride >= rows)
       return;
     float2 v[4];
     const float s = scale_value<FMT>(scale[i]);
@@ -257,9 +287,20 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const __grid_constan
       values8(v, w, s);
     }
     T *p = out + i * kStride * a.cols;
-    if constexpr (V == 8) {
-      store8<DT, VEC>(p, v, have);
-    } else if (VEC && have >= 4) {
+    if constexpr (!VEC) { // the warp's rows together: kWarpRows, from its first on
+      __shared__ uint4 scratch[kThreads / 32][kScratch / 16];
+      constexpr int kWarpRows = V / 4;
+      uint4 words[2];
+      to_words<DT, 1>(words, reinterpret_cast<const float2(&)[1][4]>(v));
+      const int64_t first = r0 - (threadIdx.x & 31) / kLanes + i * kStride, c0 = static_cast<int64_t>(tc) * kTile;
+      const int64_t there = a.rows - first, n = a.cols - c0;
+      ragged_store<Bits<DT>, V>(words, reinterpret_cast<uint8_t *>(scratch[threadIdx.x >> 5]),
+                                static_cast<Bits<DT> *>(a.out) + first * a.cols + c0, a.cols,
+                                there < kWarpRows ? static_cast<int>(there) : kWarpRows,
+                                n < kTile ? static_cast<int>(n) : kTile);
+    } else if constexpr (V == 8) {
+      store8<DT, true>(p, v, have);
+    } else if (have >= 4) {
       __stcs(reinterpret_cast<float4 *>(p), make_float4(v[0].x, v[0].y, v[1].x, v[1].y));
     } else {
       const float e[4] = {v[0].x, v[0].y, v[1].x, v[1].y};
@@ -321,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 3 : 4) k_mx_dequanti
     const int ag = t & 15, c = t >> 4; // rows 8 ag + i, columns 8 c + j
     const int64_t r = r0 + 8 * ag;
     const int have = static_cast<int>(a.rows - r < 8 ? a.rows - r : 8);
-    if (have <= 0 || c0 + 8 * c >= a.cols)
+    if (VEC && (have <= 0 || c0 + 8 * c >= a.cols))
       continue;
     // Two columns at a time from the codes' 16-bit values, which keeps the
     // registers of four blocks to an SM. What was staged for rows past the end
@@ -341,13 +382,23 @@ __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 3 : 4) k_mx_dequanti
         two[i] = __fmul2_rn(unpack2<SBC_F16>(h[i][j]), make_float2(scale[i], scale[i]));
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        if (c0 + 8 * c + 2 * j + k >= a.cols)
+        if (VEC && c0 + 8 * c + 2 * j + k >= a.cols)
           break;
-        float2 col[4];
+        float2 col[1][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          col[i] = k ? make_float2(two[2 * i].y, two[2 * i + 1].y) : make_float2(two[2 * i].x, two[2 * i + 1].x);
-        store8<DT, VEC>(static_cast<T *>(a.out) + (c0 + 8 * c + 2 * j + k) * a.rows + r, col, have);
+          col[0][i] = k ? make_float2(two[2 * i].y, two[2 * i + 1].y) : make_float2(two[2 * i].x, two[2 * i + 1].x);
+        if constexpr (VEC) {
+          store8<DT, true>(static_cast<T *>(a.out) + (c0 + 8 * c + 2 * j + k) * a.rows + r, col[0], have);
+        } else { // the warp's two columns, 8 apart, together
+          __shared__ uint4 scratch[kThreads / 32][kScratch / 16];
+          uint4 words[2];
+          to_words<DT, 1>(words, col);
+          const int64_t first = c0 + 8 * (c & ~1) + 2 * j + k, n = a.rows - r0;
+          ragged_store<Bits<DT>, 8>(words, reinterpret_cast<uint8_t *>(scratch[t >> 5]),
+                                    static_cast<Bits<DT> *>(a.out) + first * a.rows + r0, 8 * a.rows,
+                                    (first < a.cols) + (first + 8 < a.cols), n < kTile ? static_cast<int>(n) : kTile);
+        }
       }
     }
   }
@@ -371,8 +422,8 @@ template <int DT, bool VEC> int launch_quantize(const QuantizeArgs &a, int fmt, 
     k<<<grid, kThreads, 0, s>>>(a);
   } else {
     const int bytes = kTile * kTile * static_cast<int>(sizeof(typename Value<DT>::T)) + kTile * 64 + 512;
-    const cudaError_t e = a.codes ? sbc::allow_shared<k_mx_quantize_across<DT, true, VEC>>()
-                                  : sbc::allow_shared<k_mx_quantize_across<DT, false, VEC>>();
+    const cudaError_t e = a.codes ? sbc::allow_shared<k_mx_quantize_across<DT, true, VEC>>(bytes)
+                                  : sbc::allow_shared<k_mx_quantize_across<DT, false, VEC>>(bytes);
     if (e != cudaSuccess)
       return e;
     auto k = a.codes ? k_mx_quantize_across<DT, true, VEC> : k_mx_quantize_across<DT, false, VEC>;

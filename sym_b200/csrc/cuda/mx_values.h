@@ -330,4 +330,81 @@ __device__ __forceinline__ void values8(float2 (&v)[4], uint2 codes, float scale
   }
 }
 
+// Rows that do not start on 16-byte boundaries. A warp's lanes then take
+// neighbouring elements, 32 at a time, and exchange them with the owners of the
+// parts through shared memory; each lane loading or storing its own part
+// element by element would touch 32 sectors per instruction (five times slower
+// for 16-bit values, measured). A warp holds 32 V / 128 rows of 128 elements.
+
+constexpr int kScratch = 1024; // bytes per warp
+
+/// The elements of a warp's rows on their way: fetch() issues the loads,
+/// place() hands each lane the V elements of its part.
+template <typename U, int V> struct Ragged {
+  static constexpr int kRows = V / 4;
+  U e[kRows][4];
+
+  /// `rows` of the warp's rows exist, with `n` elements each from p on.
+  __device__ __forceinline__ void fetch(const U *p, int64_t stride, int rows, int n) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        e[r][j] = r < rows && lane + 32 * j < n ? __ldg(p + r * stride + lane + 32 * j) : U(0);
+  }
+  __device__ __forceinline__ void place(uint4 *part, uint8_t *scratch) const {
+    const int lane = threadIdx.x & 31;
+    U *s = reinterpret_cast<U *>(scratch);
+    __syncwarp(); // the last use of the scratch is over
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        s[r * 128 + lane + 32 * j] = e[r][j];
+    __syncwarp();
+    constexpr int kVec = V * static_cast<int>(sizeof(U)) / 16;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      part[i] = reinterpret_cast<const uint4 *>(scratch)[lane * kVec + i];
+  }
+};
+
+/// Stores the lanes' parts (V elements each, as words) to a warp's rows.
+template <typename U, int V>
+__device__ __forceinline__ void ragged_store(const uint4 *part, uint8_t *scratch, U *p, int64_t stride, int rows, int n) {
+  constexpr int kRows = V / 4, kVec = V * static_cast<int>(sizeof(U)) / 16;
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kVec; ++i)
+    reinterpret_cast<uint4 *>(scratch)[lane * kVec + i] = part[i];
+  __syncwarp();
+  const U *s = reinterpret_cast<const U *>(scratch);
+#pragma unroll
+  for (int r = 0; r < kRows; ++r)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (r < rows && lane + 32 * j < n)
+        p[r * stride + lane + 32 * j] = s[r * 128 + lane + 32 * j];
+}
+
+/// A type's bits.
+template <int DT> using Bits = typename std::conditional<DT == SBC_F32, uint32_t, uint16_t>::type;
+
+/// Values of a part as words of their type.
+template <int DT, int N> __device__ __forceinline__ void to_words(uint4 *words, const float2 (&v)[N][4]) {
+  uint32_t *w = reinterpret_cast<uint32_t *>(words);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (DT == SBC_F32) {
+        w[i * 8 + 2 * k] = __float_as_uint(v[i][k].x);
+        w[i * 8 + 2 * k + 1] = __float_as_uint(v[i][k].y);
+      } else {
+        w[i * 4 + k] = pack2<DT>(v[i][k].x, v[i][k].y);
+      }
+}
+
 } // namespace mx
