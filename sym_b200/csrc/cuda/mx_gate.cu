@@ -117,16 +117,14 @@ template <int DT> struct RaggedRows {
     ragged.fetch(static_cast<const U *>(x) + (r + unit * kStride) * stride + c0, stride, rows(a, unit), n);
   }
   __device__ __forceinline__ void store(const GateArgs &a, void *x, int64_t stride, int unit,
-                                        const float2 (&v)[Part<DT>::kValues / 8][4]) const {
-    uint4 words[2];
-    to_words<DT, Part<DT>::kValues / 8>(words, v);
+                                        const uint4 (&words)[2]) const {
     ragged_store<U, Part<DT>::kValues>(words, scratch, static_cast<U *>(x) + (r + unit * kStride) * stride + c0, stride,
                                        rows(a, unit), n);
   }
 };
 
 template <int DT, bool KEEP, bool VEC>
-__global__ void __launch_bounds__(kThreads, 3) k_silu_mul(const __grid_constant__ GateArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) k_silu_mul(const __grid_constant__ GateArgs a) {
   using T = typename Value<DT>::T;
   using P = Place<DT>;
   constexpr int N = Part<DT>::kValues / 8;
@@ -160,27 +158,28 @@ __global__ void __launch_bounds__(kThreads, 3) k_silu_mul(const __grid_constant_
   }
 #pragma unroll
   for (int i = 0; i < P::kUnits; ++i) {
-    float2 h[N][4];
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      float2 g[4], u[4];
-      gate[i].raw[j].values(g);
-      up[i].raw[j].values(u);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        h[j][k] = __fmul2_rn(__fmul2_rn(g[k], sigmoid2<DT>(g[k])), u[k]);
-    }
     const bool row_exists = p.r0 + P::kStride * i < a.rows;
-    if constexpr (!VEC)
-      ragged.store(a, a.h, a.cols, i, h);
-    else if (row_exists)
-      store_part<DT, true>(h_at + P::kStride * i * a.cols, h, p.cols);
     if (KEEP) {
       const bool exists = row_exists && p.c < a.blocks * kBlock;
       const int64_t at = block + P::kStride * i * a.blocks;
       keep<DT>(a.gate_codes, a.gate_scales, gate[i], at, p.in_block, exists);
       keep<DT>(a.up_codes, a.up_scales, up[i], at, p.in_block, exists);
     }
+    uint4 h[2];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float2 g[4], u[4], v[4];
+      gate[i].raw[j].values(g);
+      up[i].raw[j].values(u);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v[k] = __fmul2_rn(__fmul2_rn(g[k], sigmoid2<DT>(g[k])), u[k]);
+      to_words<DT>(h + j, v);
+    }
+    if constexpr (!VEC)
+      ragged.store(a, a.h, a.cols, i, h);
+    else if (row_exists)
+      store_part<DT>(h_at + P::kStride * i * a.cols, h, p.cols);
   }
 }
 
@@ -233,10 +232,10 @@ __global__ void __launch_bounds__(kThreads) k_silu_mul_backward(const __grid_con
       elements[i].place(reinterpret_cast<uint4 *>(&in[i]), ragged.scratch);
     const float gs = scale_value<SBC_MXINT8>(gate_scale[i]), us = scale_value<SBC_MXINT8>(up_scale[i]);
     const float2 one = make_float2(1.f, 1.f);
-    float2 dg[N][4], du[N][4];
+    uint4 dgate[2], dup[2];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      float2 dh[4], g[4], u[4];
+      float2 dh[4], g[4], u[4], dg[4], du[4];
       in[i].raw[j].values(dh);
       values8(g, gate[i][j], gs);
       values8(u, up[i][j], us);
@@ -244,16 +243,18 @@ __global__ void __launch_bounds__(kThreads) k_silu_mul_backward(const __grid_con
       for (int k = 0; k < 4; ++k) {
         const float2 s = sigmoid2<DT>(g[k]);
         const float2 rest = __fadd2_rn(one, make_float2(-s.x, -s.y));
-        dg[j][k] = __fmul2_rn(__fmul2_rn(dh[k], u[k]), __fmul2_rn(s, __ffma2_rn(g[k], rest, one)));
-        du[j][k] = __fmul2_rn(dh[k], __fmul2_rn(g[k], s));
+        dg[k] = __fmul2_rn(__fmul2_rn(dh[k], u[k]), __fmul2_rn(s, __ffma2_rn(g[k], rest, one)));
+        du[k] = __fmul2_rn(dh[k], __fmul2_rn(g[k], s));
       }
+      to_words<DT>(dgate + j, dg);
+      to_words<DT>(dup + j, du);
     }
     if constexpr (VEC) {
-      store_part<DT, true>(dgate_at + P::kStride * i * a.h_stride, dg, p.cols);
-      store_part<DT, true>(dup_at + P::kStride * i * a.dup_stride, du, p.cols);
+      store_part<DT>(dgate_at + P::kStride * i * a.h_stride, dgate, p.cols);
+      store_part<DT>(dup_at + P::kStride * i * a.dup_stride, dup, p.cols);
     } else {
-      ragged.store(a, a.h, a.h_stride, i, dg);
-      ragged.store(a, a.dup, a.dup_stride, i, du);
+      ragged.store(a, a.h, a.h_stride, i, dgate);
+      ragged.store(a, a.dup, a.dup_stride, i, dup);
     }
   }
 }

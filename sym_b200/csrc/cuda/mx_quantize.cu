@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const __grid_constan
       __shared__ uint4 scratch[kThreads / 32][kScratch / 16];
       constexpr int kWarpRows = V / 4;
       uint4 words[2];
-      to_words<DT, 1>(words, reinterpret_cast<const float2(&)[1][4]>(v));
+      to_words<DT>(words, v);
       const int64_t first = r0 - (threadIdx.x & 31) / kLanes + i * kStride, c0 = static_cast<int64_t>(tc) * kTile;
       const int64_t there = a.rows - first, n = a.cols - c0;
       ragged_store<Bits<DT>, V>(words, reinterpret_cast<uint8_t *>(scratch[threadIdx.x >> 5]),
@@ -384,16 +384,16 @@ __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 3 : 4) k_mx_dequanti
       for (int k = 0; k < 2; ++k) {
         if (VEC && c0 + 8 * c + 2 * j + k >= a.cols)
           break;
-        float2 col[1][4];
+        float2 col[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          col[0][i] = k ? make_float2(two[2 * i].y, two[2 * i + 1].y) : make_float2(two[2 * i].x, two[2 * i + 1].x);
+          col[i] = k ? make_float2(two[2 * i].y, two[2 * i + 1].y) : make_float2(two[2 * i].x, two[2 * i + 1].x);
         if constexpr (VEC) {
-          store8<DT, true>(static_cast<T *>(a.out) + (c0 + 8 * c + 2 * j + k) * a.rows + r, col[0], have);
+          store8<DT, true>(static_cast<T *>(a.out) + (c0 + 8 * c + 2 * j + k) * a.rows + r, col, have);
         } else { // the warp's two columns, 8 apart, together
           __shared__ uint4 scratch[kThreads / 32][kScratch / 16];
           uint4 words[2];
-          to_words<DT, 1>(words, col);
+          to_words<DT>(words, col);
           const int64_t first = c0 + 8 * (c & ~1) + 2 * j + k, n = a.rows - r0;
           ragged_store<Bits<DT>, 8>(words, reinterpret_cast<uint8_t *>(scratch[t >> 5]),
                                     static_cast<Bits<DT> *>(a.out) + first * a.rows + r0, 8 * a.rows,

@@ -207,25 +207,39 @@ template <int DT> struct Part {
   }
 };
 
-/// Stores a part's values, of which `have` exist.
-template <int DT, bool VEC>
-__device__ __forceinline__ void store_part(typename Value<DT>::T *p, const float2 (&v)[Part<DT>::kValues / 8][4], int have) {
-  constexpr int V = Part<DT>::kValues;
-  if (VEC && have >= V && reinterpret_cast<uintptr_t>(p) % 32 == 0) {
-    uint32_t w[8];
+/// The eight values v in their type, as words.
+template <int DT> __device__ __forceinline__ void to_words(uint4 *words, const float2 (&v)[4]) {
+  uint32_t *w = reinterpret_cast<uint32_t *>(words);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (DT == SBC_F32)
-        w[i] = __float_as_uint(i & 1 ? v[0][i / 2].y : v[0][i / 2].x);
-      else
-        w[i] = pack2<DT>(v[i / 4 % (V / 8)][i & 3].x, v[i / 4 % (V / 8)][i & 3].y);
+  for (int k = 0; k < 4; ++k)
+    if (DT == SBC_F32) {
+      w[2 * k] = __float_as_uint(v[k].x);
+      w[2 * k + 1] = __float_as_uint(v[k].y);
+    } else {
+      w[k] = pack2<DT>(v[k].x, v[k].y);
+    }
+}
+
+/// Stores a part's values (32 bytes), of which `have` exist; p is 16-byte
+/// aligned.
+template <int DT>
+__device__ __forceinline__ void store_part(typename Value<DT>::T *p, const uint4 (&q)[2], int have) {
+  constexpr int V = Part<DT>::kValues;
+  const uint32_t *w = reinterpret_cast<const uint32_t *>(q);
+  if (have >= V && reinterpret_cast<uintptr_t>(p) % 32 == 0) {
     asm volatile("st.global.cs.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                  "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                  : "memory");
+  } else if (have >= V) {
+    __stcs(reinterpret_cast<uint4 *>(p), q[0]);
+    __stcs(reinterpret_cast<uint4 *>(p) + 1, q[1]);
   } else {
+    using U = typename std::conditional<DT == SBC_F32, uint32_t, uint16_t>::type;
+    U *u = reinterpret_cast<U *>(p);
 #pragma unroll
-    for (int i = 0; i < V / 8; ++i)
-      store8<DT, VEC>(p + 8 * i, v[i], have - 8 * i);
+    for (int i = 0; i < V; ++i)
+      if (i < have)
+        u[i] = DT == SBC_F32 ? static_cast<U>(w[i & 7]) : static_cast<U>(w[i / 2 & 7] >> (i & 1) * 16);
   }
 }
 
@@ -391,20 +405,5 @@ __device__ __forceinline__ void ragged_store(const uint4 *part, uint8_t *scratch
 
 /// A type's bits.
 template <int DT> using Bits = typename std::conditional<DT == SBC_F32, uint32_t, uint16_t>::type;
-
-/// Values of a part as words of their type.
-template <int DT, int N> __device__ __forceinline__ void to_words(uint4 *words, const float2 (&v)[N][4]) {
-  uint32_t *w = reinterpret_cast<uint32_t *>(words);
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (DT == SBC_F32) {
-        w[i * 8 + 2 * k] = __float_as_uint(v[i][k].x);
-        w[i * 8 + 2 * k + 1] = __float_as_uint(v[i][k].y);
-      } else {
-        w[i * 4 + k] = pack2<DT>(v[i][k].x, v[i][k].y);
-      }
-}
 
 } // namespace mx
