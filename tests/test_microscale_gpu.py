@@ -432,7 +432,8 @@ def test_feed_forward_together():
     check_product(down.grad, O.rounded(dyh.T), O.rounded(h.T))
     dh = mx.matmul(mx.quantize(dy), mx.quantize(down, along=0), dtype=torch.bfloat16)
     gq, uq = O.rounded(a[:, :352], "mxint8"), O.rounded(a[:, 352:], "mxint8")
-    s = 1 / (1 + np.exp(-gq))
+    with np.errstate(over="ignore"):
+        s = 1 / (1 + np.exp(-gq))
     da = torch.from_numpy(np.concatenate((host(dh) * uq * s * (1 + gq * (1 - s)), host(dh) * gq * s), 1)).to(torch.bfloat16)
     got, = torch.autograd.grad(mx.silu_mul(t := torch.from_numpy(a).to(torch.bfloat16).cuda().requires_grad_()), t, dh)
     step = 2.0 ** -7  # the two may round to neighbouring values
@@ -513,3 +514,97 @@ def test_gpu_refusals_leave_the_device_usable():
     with pytest.raises(TypeError):
         mx.linear(x, q, dtype=torch.float64)
     assert mx.linear(x, q).isfinite().all()
+
+
+def test_two_graphs_of_one_memory_pool():
+    """Graphs that share a pool, and so each other's freed workspaces, replayed
+    in turn."""
+    xs = [tensor((m, 1024), torch.bfloat16, 60 + m) for m in (40, 200)]
+    w = mx.quantize(tensor((640, 1024), torch.float32, 61, 0.05))
+    want = [mx.silu_mul(mx.linear(x, w)) for x in xs]
+    pool = torch.cuda.graph_pool_handle()
+    graphs = []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            out = mx.silu_mul(mx.linear(x, w))
+        graphs.append((g, out))
+    for turn in (0, 1, 1, 0):
+        graphs[turn][0].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(graphs[turn][1], want[turn])
+
+
+def test_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from sym_b200 import microscale as mx
+x = torch.ones(20, 64, device="cuda", dtype=torch.bfloat16)
+codes = torch.full((96, 32), 0x22, dtype=torch.uint8, device="cuda")  # ones
+w = mx.MxTensor(codes, torch.full((512,), 127, dtype=torch.uint8, device="cuda"), (96, 64))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = mx.linear(x, w)
+    z = mx.linear(x[:1], w)
+    q, qt = mx.quantize_both(x)
+g.replay()
+torch.cuda.synchronize()
+assert (y == 64).all() and (z == 64).all() and (mx.dequantize(qt) == 1).all()
+"""
+    root = Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_second_derivatives_are_refused():
+    x, w = tensor((8, 64), torch.float32, 62).requires_grad_(), tensor((32, 64), torch.float32, 63).requires_grad_()
+    for y in (mx.linear(x, w), mx.silu_mul(x, x * 2)):
+        g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)
+
+
+def test_training_product_of_one_row_and_of_a_transposed_weight():
+    x, w = tensor((64,), torch.float16, 64).requires_grad_(), tensor((64, 40), torch.float16, 65).requires_grad_()
+    y = mx.linear(x, w.t())
+    dy = tensor((40,), torch.float16, 66)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert y.shape == (40,) and dx.shape == (64,) and dw.shape == (64, 40)
+    row, wt = host(x)[None], host(w).T
+    check_product(y[None], O.rounded(row), O.rounded(wt))
+    check_product(dx[None], O.rounded(host(dy)[None]), O.rounded(wt.T))
+    check_product(dw.t(), O.rounded(host(dy)[None].T), O.rounded(row.T))
+
+
+def test_large_offsets():
+    """Codes, values and results beyond 2^31 elements: the last rows agree with
+    the same rows alone."""
+    rows, cols = 70_000, 32_768
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[:-3].fill_(1.0)
+    x[-3:] = tensor((3, cols), torch.bfloat16, 67)
+    q, qt = mx.quantize_both(x)
+    alone = mx.quantize(x[-3:])
+    assert torch.equal(q.codes[-3:], alone.codes)
+    last = mx.dequantize(q, torch.bfloat16)[-3:]
+    assert torch.equal(last, mx.dequantize(alone, torch.bfloat16))
+    del q
+    # the transposed form: the last block of every column holds the last rows
+    tail = mx.quantize(x[-(rows % 32 or 32):], along=0)
+    assert torch.equal(qt.codes[:, -16:], tail.codes)
+    wide = mx.dequantize(qt, torch.bfloat16, transpose=True)
+    assert torch.equal(wide[-3:], mx.dequantize(tail, torch.bfloat16, transpose=True)[-3:])
+    del wide, qt
+    h = mx.silu_mul(x, x)
+    assert torch.equal(h[-3:], mx.silu_mul(x[-3:], x[-3:]))
+    del h
+    w = mx.quantize(tensor((64, cols), torch.bfloat16, 68, 0.05))
+    y = mx.linear(x, w)
+    assert torch.equal(mx.linear(x[-300:], w)[-3:], mx.linear(x[-300:].clone(), w)[-3:])
+    a, b = O.rounded(host(x[-3:])), O.rounded(host(tensor((64, cols), torch.bfloat16, 68, 0.05)))
+    check_product(y[-3:], a, b)
