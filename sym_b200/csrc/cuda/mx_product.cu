@@ -186,20 +186,43 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
   using S = Shape<NT, FUSED>;
   using T = typename Value<DT>::T;
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t full[S::kStages], empty[S::kStages], ready, quantized;
+  __shared__ uint64_t full[S::kStages], empty[S::kStages], ready;
   __shared__ uint32_t tmem_base;
   const uint32_t stage0 = (smem_addr(raw) + 1023) & ~1023u;
   const uint32_t own_a = stage0 + S::kStages * S::kStage; // FUSED: the codes of all steps, then the scales
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+  const uint32_t tile = blockIdx.x / a.split, rank = blockIdx.x - tile * a.split;
+  const uint32_t tb = tile / a.tiles_a, ta = tile - tb * a.tiles_a;
+  const uint32_t ks0 = a.steps * rank / a.split, ks1 = a.steps * (rank + 1) / a.split;
+  const int64_t m0 = static_cast<int64_t>(ta) * NT;
+  const int cols = static_cast<int>(a.m - m0 < NT ? a.m - m0 : NT);
+  const int first = static_cast<int>(ks1 - ks0 < S::kStages ? ks1 - ks0 : S::kStages); // stages of the first round
+
+  const auto scale_bytes = [&](uint32_t ks) { return (a.quads - 2 * ks < 2 ? 1u : 2u) * 512u; };
+  const auto load_b = [&](uint32_t ks, int st) {
+    const uint32_t at = stage0 + st * S::kStage, bar = smem_addr(&full[st]);
+    expect_bytes(bar, S::kBytesB + S::kBytesA + (FUSED ? 1 : 2) * scale_bytes(ks));
+    if (!(a.withhold && blockIdx.x == 0 && ks == ks0))
+      load_box(at, &a.map_b, ks * 128, tb * kRowsB, bar);
+    load_bytes(at + S::kScales, a.scales_b + (static_cast<int64_t>(tb) * a.quads + 2 * static_cast<int64_t>(ks)) * 512,
+               scale_bytes(ks), bar);
+  };
+
+  // The first weights are on their way before anything else: they wait neither
+  // for tensor memory nor for the kernel that quantises A.
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < S::kStages; ++i) {
+        mbar_init(&full[i], 1);
+        mbar_init(&empty[i], 1);
+      }
+      mbar_init(&ready, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    mbar_init(&ready, 1);
-    mbar_init(&quantized, 128);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
+    for (int st = 0; st < first; ++st)
+      load_b(ks0 + st, st);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
@@ -207,27 +230,61 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  if constexpr (FUSED) if (warp >= 2) {
+    const int t = threadIdx.x - 64;
+    // 8 values of one row per unit, four lanes a block, 32 units of a row a
+    // step; 1, 2 or 4 rows at a time, so that a part of one or two steps
+    // keeps all warps busy. The loads of a group of units come before its
+    // first use.
+    const typename Value<XT>::T *x = static_cast<const typename Value<XT>::T *>(a.x);
+    const int in_row = static_cast<int>(ks1 - ks0) * 32;
+    const int lg = in_row <= 32 ? 5 : in_row <= 64 ? 6 : 7;
+    const uint32_t scales = own_a + (ks1 - ks0) * S::kStepA;
+    for (int row = t >> lg; row < cols; row += 128 >> lg) {
+      const typename Value<XT>::T *p = x + (m0 + row) * a.x_stride;
+      for (int at0 = t & ((1 << lg) - 1); at0 < in_row; at0 += kUnits << lg) {
+        Raw8<XT> in[kUnits];
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          const int at = at0 + (i << lg);
+          const int64_t c = static_cast<int64_t>(ks0) * kStep + at * 8;
+          const int have = at >= in_row || c >= a.k ? 0 : static_cast<int>(a.k - c < 8 ? a.k - c : 8);
+          if (a.x_vec)
+            in[i].template load<true>(p + c, have);
+          else
+            in[i].template load<false>(p + c, have);
+        }
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          const int at = at0 + (i << lg);
+          if (at >= in_row) // whole warps
+            break;
+          const int step = at >> 5, kk = (at & 31) * 8;
+          const uint32_t byte = scale_byte<SBC_MXFP4>(top_of_lanes<2>(in[i].top()));
+          float2 v[4];
+          in[i].values(v);
+          times(v, inverse_scale<SBC_MXFP4>(byte));
+          const uint32_t w = byte == 255 ? 0 : codes4(v);
+          // the 128-byte swizzle: 16-byte chunk kk / 32 of row r lies at chunk (kk / 32) ^ (r mod 8)
+          const uint32_t code_at =
+              own_a + step * S::kStepA + row * 128 + (((kk >> 5) ^ (row & 7)) << 4) + (kk >> 1 & 15);
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(code_at), "r"(w) : "memory");
+          if ((lane & 3) == 0)
+            asm volatile("st.shared.u8 [%0], %1;" ::"r"(scales + step * S::kScaleA + (kk >> 7) * S::kTileA +
+                                                        row * 16 + (kk >> 5 & 3)),
+                         "r"(byte)
+                         : "memory");
+        }
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = __shfl_sync(~0u, tmem_base, 0);
-  const uint32_t tile = blockIdx.x / a.split, rank = blockIdx.x - tile * a.split;
-  const uint32_t tb = tile / a.tiles_a, ta = tile - tb * a.tiles_a;
-  const uint32_t ks0 = a.steps * rank / a.split, ks1 = a.steps * (rank + 1) / a.split;
-  const int64_t m0 = static_cast<int64_t>(ta) * NT;
-  const int cols = static_cast<int>(a.m - m0 < NT ? a.m - m0 : NT);
-
   if (warp == 0) {
-    const uint8_t *sb = a.scales_b + static_cast<int64_t>(tb) * a.quads * 512;
     const uint8_t *sa = FUSED ? nullptr : a.scales_a + m0 / 128 * a.quads * 512;
-    const auto scale_bytes = [&](uint32_t ks) { return (a.quads - 2 * ks < 2 ? 1u : 2u) * 512u; };
-    const auto load_b = [&](uint32_t ks, int st) {
-      const uint32_t at = stage0 + st * S::kStage, bar = smem_addr(&full[st]);
-      expect_bytes(bar, S::kBytesB + S::kBytesA + (FUSED ? 1 : 2) * scale_bytes(ks));
-      if (!(a.withhold && blockIdx.x == 0 && ks == ks0))
-        load_box(at, &a.map_b, ks * 128, tb * kRowsB, bar);
-      load_bytes(at + S::kScales, sb + static_cast<int64_t>(ks) * 1024, scale_bytes(ks), bar);
-    };
     const auto load_a = [&](uint32_t ks, int st) {
       if (FUSED)
         return;
@@ -235,11 +292,6 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
       load_box(at + S::kBytesB, &a.map_a, ks * 128, static_cast<int32_t>(m0), bar);
       load_bytes(at + S::kScales + kScaleStage, sa + static_cast<int64_t>(ks) * 1024, scale_bytes(ks), bar);
     };
-    // The first round of stages: the weights' loads do not wait for the
-    // kernel that quantises A.
-    const int first = static_cast<int>(ks1 - ks0 < S::kStages ? ks1 - ks0 : S::kStages);
-    for (int st = 0; st < first; ++st)
-      load_b(ks0 + st, st);
     if (!FUSED && a.after_quantize)
       asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int st = 0; st < first; ++st)
@@ -288,7 +340,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
       }
       return true;
     };
-    bool ok = (!FUSED || warp_wait(&quantized, 0, a.wait_ns)) && scales(ks0);
+    bool ok = scales(ks0);
     for (uint32_t ks = ks0; ks < ks1 && ok; ++ks) {
       if (ks + 1 < ks1)
         ok = scales(ks + 1);
@@ -312,58 +364,8 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
       warp_wait(&ready, 0, a.wait_ns);
     }
   } else {
-    const int t = threadIdx.x - 64;
-    if (FUSED) {
-      // 8 values of one row per unit, four lanes a block, 32 units of a row a
-      // step; 1, 2 or 4 rows at a time, so that a part of one or two steps
-      // keeps all warps busy. The loads of a group of units come before its
-      // first use.
-      const typename Value<XT>::T *x = static_cast<const typename Value<XT>::T *>(a.x);
-      const int in_row = static_cast<int>(ks1 - ks0) * 32;
-      const int lg = in_row <= 32 ? 5 : in_row <= 64 ? 6 : 7;
-      const uint32_t scales = own_a + (ks1 - ks0) * S::kStepA;
-      for (int row = t >> lg; row < cols; row += 128 >> lg) {
-        const typename Value<XT>::T *p = x + (m0 + row) * a.x_stride;
-        for (int at0 = t & ((1 << lg) - 1); at0 < in_row; at0 += kUnits << lg) {
-          Raw8<XT> in[kUnits];
-#pragma unroll
-          for (int i = 0; i < kUnits; ++i) {
-            const int at = at0 + (i << lg);
-            const int64_t c = static_cast<int64_t>(ks0) * kStep + at * 8;
-            const int have = at >= in_row || c >= a.k ? 0 : static_cast<int>(a.k - c < 8 ? a.k - c : 8);
-            if (a.x_vec)
-              in[i].template load<true>(p + c, have);
-            else
-              in[i].template load<false>(p + c, have);
-          }
-#pragma unroll
-          for (int i = 0; i < kUnits; ++i) {
-            const int at = at0 + (i << lg);
-            if (at >= in_row) // whole warps
-              break;
-            const int step = at >> 5, kk = (at & 31) * 8;
-            const uint32_t byte = scale_byte<SBC_MXFP4>(top_of_lanes<2>(in[i].top()));
-            float2 v[4];
-            in[i].values(v);
-            times(v, inverse_scale<SBC_MXFP4>(byte));
-            const uint32_t w = byte == 255 ? 0 : codes4(v);
-            // the 128-byte swizzle: 16-byte chunk kk / 32 of row r lies at chunk (kk / 32) ^ (r mod 8)
-            const uint32_t code_at =
-                own_a + step * S::kStepA + row * 128 + (((kk >> 5) ^ (row & 7)) << 4) + (kk >> 1 & 15);
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(code_at), "r"(w) : "memory");
-            if ((lane & 3) == 0)
-              asm volatile("st.shared.u8 [%0], %1;" ::"r"(scales + step * S::kScaleA + (kk >> 7) * S::kTileA +
-                                                          row * 16 + (kk >> 5 & 3)),
-                           "r"(byte)
-                           : "memory");
-          }
-        }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(&quantized);
-    } else if (a.after_quantize) {
+    if (!FUSED && a.after_quantize)
       asm volatile("griddepcontrol.wait;" ::: "memory");
-    }
     const int quarter = warp & 3; // the lanes of tensor memory that this warp may read
     const int row = quarter * 32 + lane;
     const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
