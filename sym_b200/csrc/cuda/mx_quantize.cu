@@ -1,8 +1,20 @@
 // sym_b200 -- microscaled quantisation and its inverse (formats: mx_values.h).
 //
-// One block of threads takes a tile of 128 rows x 128 columns, which is one
-// 512-byte scale tile in either direction. All kernels are bound by memory:
-// they read each value once and write each code once.
+// One block of threads takes a tile of 128 columns, 64 or 128 rows: with 128
+// rows one 512-byte scale tile in either direction. All kernels are bound by
+// memory: they read each value once and write each code once. What it takes
+// to get there: loads of all of a thread's parts before the first use, 32
+// bytes per thread (one sector), magnitudes compared as packed whole numbers,
+// scaling in packed 32-bit pairs, no 64-bit division per part.
+//
+// Measured (8192 x 8192, captured back to back; bytes of the task over time):
+//   rows, f16 26.2 us = 6.5 TB/s, f32 45.3 us = 6.7; both directions in one
+//   read, f16 40.1 us = 5.1, f32 68.5 us = 5.0 (the issue of the second
+//   direction's instructions, 66 % busy); across alone, f16 40.6 us = 4.2;
+//   back to values, f16 26.3 us = 6.5, f32 47.7 us = 6.4, transposed f16
+//   30.2 us = 5.6. [28672, 8192] to f16 [in, out]: 111 us = 5.4.
+//   Rows of 8191 columns (through shared memory per warp): f16 39.4, 59.8 and,
+//   back, 36.7 us; each lane by itself 53, 80 and 196.
 #include "barriers.h"
 #include "mx_values.h"
 
