@@ -93,9 +93,16 @@ class MxTensor:
     and uint8 ``scales`` (flat, in the format's order).
 
     The constructor takes tensors that already have that layout, without a
-    copy; ``from_rows`` takes row-major scales, as checkpoints hold them."""
+    copy; ``from_rows`` takes row-major scales, as checkpoints hold them. A
+    matrix keeps its tensors; they are not exchanged for others (``native``
+    holds their addresses), but copies and pickles are made from them."""
 
-    __slots__ = ("codes", "scales", "shape", "format", "native")
+    __slots__ = ("_codes", "_scales", "_shape", "_format", "_native")
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    shape = property(lambda self: self._shape)
+    format = property(lambda self: self._format)
+    native = property(lambda self: self._native)
 
     def __init__(self, codes, scales, shape, format="mxfp4"):
         if format not in FORMATS:
@@ -113,25 +120,28 @@ class MxTensor:
         if scales.numel() != _scale_bytes(rows, cols, format) or not scales.is_contiguous():
             raise ValueError(f"{format} scales of [{rows}, {cols}] are {_scale_bytes(rows, cols, format)} "
                              "contiguous bytes")
-        self.codes, self.scales, self.shape, self.format = codes, scales, (rows, cols), format
-        self.native = None
+        self._codes, self._scales, self._shape, self._format = codes, scales, (rows, cols), format
+        self._native = None
         if codes.is_cuda and rows:
             if codes.data_ptr() % 16 or scales.data_ptr() % 16:
                 raise ValueError("codes and scales start on 16-byte boundaries")
-            self.native = _native.SbMx(codes.data_ptr(), scales.data_ptr(), rows, cols, FORMATS[format],
+            self._native = _native.SbMx(codes.data_ptr(), scales.data_ptr(), rows, cols, FORMATS[format],
                                        codes.device.index)
 
     @classmethod
     def _empty(cls, like, rows, cols, format="mxfp4"):
         """An uninitialised matrix on the device of ``like``."""
         q = cls.__new__(cls)
-        q.codes = like.new_empty((rows, _blocks(cols) * _CODE_BYTES[format]), dtype=torch.uint8)
-        q.scales = like.new_empty(_scale_bytes(rows, cols, format), dtype=torch.uint8)
-        q.shape, q.format, q.native = (rows, cols), format, None
+        q._codes = codes = like.new_empty((rows, _blocks(cols) * _CODE_BYTES[format]), dtype=torch.uint8)
+        q._scales = scales = like.new_empty(_scale_bytes(rows, cols, format), dtype=torch.uint8)
+        q._shape, q._format, q._native = (rows, cols), format, None
         if rows:
-            q.native = _native.SbMx(q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, FORMATS[format],
-                                    like.get_device())
+            q._native = _native.SbMx(codes.data_ptr(), scales.data_ptr(), rows, cols, FORMATS[format],
+                                     like.get_device())
         return q
+
+    def __reduce__(self):
+        return MxTensor, (self._codes, self._scales, self._shape, self._format)
 
     @classmethod
     def from_rows(cls, codes, row_scales, cols, format="mxfp4"):
@@ -155,10 +165,10 @@ class MxTensor:
 
     @property
     def device(self):
-        return self.codes.device
+        return self._codes.device
 
     def get_device(self):
-        return self.codes.get_device()
+        return self._codes.get_device()
 
     def to(self, device, non_blocking=False):
         return MxTensor(self.codes.to(device, non_blocking=non_blocking),
@@ -342,7 +352,7 @@ def _linear(x, w, dtype):
         index = x.get_device()
         size = _linear_workspace(m, n, k, index)
         space = x.new_empty(size, dtype=torch.uint8) if size else None
-        _check(_lib().sb_mx_linear(x.data_ptr(), _DTYPES[x.dtype], m, stride, w.native, y.data_ptr(), _DTYPES[dtype],
+        _check(_lib().sb_mx_linear(x.data_ptr(), _DTYPES[x.dtype], m, stride, w._native, y.data_ptr(), _DTYPES[dtype],
                                    space.data_ptr() if size else None, size, _stream(index), _scratch.ref))
     return y
 
@@ -373,6 +383,8 @@ class _TrainLinear(torch.autograd.Function):
         n, k = weight.shape
         m = x.numel() // k
         ctx.dtypes, ctx.shape, ctx.extents = (x.dtype, weight.dtype), x.shape, (m, n, k)
+        if m == 0 or n == 0:  # no rows, or no columns of the result: gradients of zeros
+            return x.new_empty((*x.shape[:-1], n), dtype=dtype)
         size, places = _layout((m, k, "mxfp4"), (n, k, "mxfp4"))
         now = x.new_empty(size, dtype=torch.uint8)
         qx, qw = _placed(now, places)
@@ -389,6 +401,9 @@ class _TrainLinear(torch.autograd.Function):
     def backward(ctx, dy):
         need_x, need_w, _ = ctx.needs_input_grad
         m, n, k = ctx.extents
+        if m == 0 or n == 0:
+            return (dy.new_zeros(ctx.shape, dtype=ctx.dtypes[0]) if need_x else None,
+                    dy.new_zeros((n, k), dtype=ctx.dtypes[1]) if need_w else None, None)
         kept, = ctx.saved_tensors
         qxt, qwt = _placed(kept, ctx.places)
         size, places = _layout((m, n, "mxfp4") if need_x else None, (n, m, "mxfp4") if need_w else None)
@@ -433,8 +448,6 @@ def linear(x, weight, weight_t=None, *, dtype=None):
         if _mx(weight_t, "weight_t", "mxfp4").shape != (k, n) or weight_t.device != x.device:
             raise ValueError(f"weight_t is [{k}, {n}] on {x.device}")
         return _FrozenLinear.apply(x, weight, weight_t, dtype)
-    if n == 0 or x.numel() == 0:
-        raise ValueError("a training product needs at least one row of x and of weight")
     return _TrainLinear.apply(x, weight, dtype)
 
 

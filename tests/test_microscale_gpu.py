@@ -507,7 +507,7 @@ def test_gpu_refusals_leave_the_device_usable():
                  lambda: mx.quantize(x, "mxint8", along=0), lambda: mx.quantize(x, along=1),
                  lambda: mx.quantize(x[0], along=0), lambda: mx.quantize(x, "fp4"), lambda: mx.quantize_both(x[:0]),
                  lambda: mx.silu_mul(x, w), lambda: mx.silu_mul(x, x.float()), lambda: mx.silu_mul(x[:, :63]),
-                 lambda: mx.linear(x[:, :0], q), lambda: mx.linear(x[:0], w), lambda: mx.linear(x, w.cpu()),
+                 lambda: mx.linear(x[:, :0], q), lambda: mx.linear(x, w.cpu()),
                  lambda: mx.MxTensor(q.codes.view(-1)[1:-31].view(-1, 32), q.scales, (79, 64))):
         with pytest.raises(ValueError):
             call()
@@ -608,3 +608,39 @@ def test_large_offsets():
     assert torch.equal(mx.linear(x[-300:], w)[-3:], mx.linear(x[-300:].clone(), w)[-3:])
     a, b = O.rounded(host(x[-3:])), O.rounded(host(tensor((64, cols), torch.bfloat16, 68, 0.05)))
     check_product(y[-3:], a, b)
+
+
+def test_training_product_without_rows():
+    """A batch of no rows (an expert that got no tokens): empty result, zero
+    weight gradient."""
+    w = tensor((40, 64), torch.bfloat16, 70).requires_grad_()
+    for shape in ((0, 64), (2, 0, 64)):
+        x = torch.empty(shape, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        y = mx.linear(x, w)
+        dx, dw = torch.autograd.grad(y, (x, w), torch.empty_like(y))
+        assert y.shape == (*shape[:-1], 40) and dx.shape == shape and torch.equal(dw, torch.zeros_like(w))
+        q, qt = mx.quantize_both(w)
+        assert torch.autograd.grad(mx.linear(x, q, qt).sum(), x)[0].shape == shape
+    g = torch.empty(0, 64, device="cuda", requires_grad=True)
+    assert torch.autograd.grad(mx.silu_mul(g, g).sum(), g)[0].shape == (0, 64)
+
+
+def test_copies_of_a_matrix_own_their_memory():
+    import copy
+    import pickle
+
+    x = tensor((5, 256), torch.float16, 71)
+    q = mx.quantize(tensor((300, 256), torch.float32, 72))
+    want = mx.linear(x, q)
+    copies = [copy.deepcopy(q), pickle.loads(pickle.dumps(q)), q.to("cpu").to("cuda"), copy.copy(q)]
+    for c in copies[:3]:
+        assert c.codes.data_ptr() != q.codes.data_ptr()
+        c_native = c.native
+        assert c_native.codes == c.codes.data_ptr() and c_native.scales == c.scales.data_ptr()
+    for name in ("codes", "scales", "shape", "format", "native"):
+        with pytest.raises(AttributeError):
+            setattr(q, name, None)
+    del q
+    torch.cuda.empty_cache()
+    for c in copies:
+        assert torch.equal(mx.linear(x, c), want)
