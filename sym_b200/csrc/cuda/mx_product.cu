@@ -836,12 +836,14 @@ struct Plan {
 ///
 /// More rows: pairs of SMs with 256, 192 or 128 rows of A a tile, or the tiles of
 /// one CTA with their split. The cost of each is the rounds of tiles that the
-/// SMs need times a tile's cycles, which are fits to measured times (steps of
-/// 700, 600, 520 and 700 cycles, and what a tile costs beside them); over 36
-/// shapes the choice by them loses 0.2 % against the best of the four. Measured,
-/// us, pairs of 256 / 192 / 128 / single CTAs: 2048 x 11008 x 4096 43.7 / 47.6 /
-/// 58.6 / 82.7; 512 x 11008 x 4096 21.9 / 20.7 / 22.8 / 32.7; 256 x 4096 x 4096
-/// 13.0 / 11.9 / 11.3 / 12.2; 256 x 1024 x 8192 23.4 / 21.5 / 17.9 / 12.6.
+/// SMs need times a tile's cycles: its steps, the change to the next tile, and no
+/// less than its results take to store. The cycles are fits to measured times;
+/// over 48 shapes the choice by them loses 0.2 % against the best of the four.
+/// Measured, us, pairs of 256 / 192 / 128 / single CTAs, with given codes: 11008 x
+/// 4096 x 2048 51.2 / 46.5 / 56.3 / 109; 2048 x 11008 x 4096 38.5 / 44.0 / 55.0 /
+/// 75.6; 1003 x 8192 x 1024 10.8 / 12.0 / 13.0 / 19.9; 1003 x 1024 x 8192 16.0 /
+/// 15.4 / 14.9 / 12.3; quantised in the call, 256 x 4096 x 4096 13.0 / 11.9 / 11.3 /
+/// 12.2; 256 x 1024 x 8192 23.4 / 21.5 / 17.9 / 12.6.
 bool plan_of(int64_t m, int64_t n, int64_t k, int sms, Plan *p) {
   p->nt = m <= 8 ? 8 : m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
   p->tiles_a = (m + p->nt - 1) / p->nt;
@@ -864,12 +866,14 @@ bool plan_of(int64_t m, int64_t n, int64_t k, int sms, Plan *p) {
   p->fused = m <= 8 && m * each <= 8;
   p->pair = 0;
   if (m > 128) {
-    const double ctas = static_cast<double>(tiles * p->split) / sms;
-    double best = (ctas < 1 ? 1 : ctas) * each * 700 + 6000;
-    const struct { int rows, step, tile; } pairs[] = {{256, 700, 2500}, {192, 600, 2500}, {128, 520, 2000}};
+    const double ctas = static_cast<double>(tiles * p->split) / sms, full = ctas < 1 ? 1 : ctas;
+    double best = full * each * 480 + (full < 2 ? 1 : full / 2) * 6000;
+    const struct { int rows, step, change, least; } pairs[] = {
+        {256, 511, 3350, 4700}, {192, 522, 1350, 4000}, {128, 505, 720, 3240}};
     for (const auto &c : pairs) {
       const int64_t t = (m + c.rows - 1) / c.rows * ((n + 255) / 256), rounds = (t + sms / 2 - 1) / (sms / 2);
-      const double cost = static_cast<double>(rounds) * (p->steps * c.step + c.tile);
+      const int64_t tile = p->steps * c.step + c.change;
+      const double cost = static_cast<double>(rounds) * (tile < c.least ? c.least : tile);
       if (cost < best) {
         best = cost;
         p->pair = c.rows;
