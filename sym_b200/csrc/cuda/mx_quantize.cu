@@ -12,7 +12,8 @@
 //   read, f16 40.1 us = 5.1, f32 68.5 us = 5.0 (the issue of the second
 //   direction's instructions, 66 % busy); across alone, f16 40.6 us = 4.2;
 //   back to values, f16 26.3 us = 6.5, f32 47.7 us = 6.4, transposed f16
-//   30.2 us = 5.6. [28672, 8192] to f16 [in, out]: 111 us = 5.4.
+//   30.2 us = 5.6, f32 56 us = 5.4. [28672, 8192] to [in, out]: f16 111 us = 5.4,
+//   f32 184 us = 5.8.
 //   Rows of 8191 columns (through shared memory per warp): f16 39.4, 59.8 and,
 //   back, 36.7 us; each lane by itself 53, 80 and 196.
 #include "barriers.h"
@@ -329,8 +330,10 @@ __global__ void __launch_bounds__(kThreads) k_mx_dequantize(const __grid_constan
 /// reads one word (8 columns) of each of 8 consecutive rows, the lanes of a
 /// warp 16 row groups x 2 words on 32 distinct banks, and writes 8 values of
 /// each column as one run (128 values of a column per half-warp).
-/// A block takes every gridDim-th tile; the next tile's codes and scales are
-/// on their way to registers while this one's values are stored.
+/// A block takes every gridDim-th tile (16-bit values; one tile with 32-bit
+/// ones); the next tile's codes and scales are on their way to registers while
+/// this one's values are stored. A lane's eight 32-bit values are stored as one
+/// sector: as two halves, [28672, 8192] took 213 us instead of 184.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 3 : 4) k_mx_dequantize_t(const __grid_constant__ DequantizeArgs a) {
   using T = typename Value<DT>::T;
@@ -400,7 +403,11 @@ __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 3 : 4) k_mx_dequanti
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           col[i] = k ? make_float2(two[2 * i].y, two[2 * i + 1].y) : make_float2(two[2 * i].x, two[2 * i + 1].x);
-        if constexpr (VEC) {
+        if constexpr (VEC && DT == SBC_F32) {
+          uint4 words[2];
+          to_words<DT>(words, col);
+          store_part<DT>(static_cast<T *>(a.out) + (c0 + 8 * c + 2 * j + k) * a.rows + r, words, have);
+        } else if constexpr (VEC) {
           store8<DT, true>(static_cast<T *>(a.out) + (c0 + 8 * c + 2 * j + k) * a.rows + r, col, have);
         } else { // the warp's two columns, 8 apart, together
           __shared__ uint4 scratch[kThreads / 32][kScratch / 16];
@@ -506,14 +513,17 @@ int sbc_mx_dequantize(const sbc_mx *q, void *out, int32_t dtype, int32_t transpo
       dtype > SBC_BF16 || !grid_of(q->rows, q->cols, transpose ? kTile : few ? (dtype == SBC_F32 ? 8 : 16) : 64, &a.tiles_c, &grid))
     return SBC_EINVAL;
   a.tiles = grid;
-  if (transpose) { // the blocks that stay on the SMs
+  // Transposed 16-bit values: the blocks that stay on the SMs, each with the next
+  // tile's codes on their way ([28672, 8192] 111 us, one block per tile 120).
+  // 32-bit values: one block per tile (184 us, four staying blocks an SM 222).
+  if (transpose && dtype != SBC_F32) {
     int device = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess)
       e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess)
       return e;
-    const uint32_t stay = static_cast<uint32_t>(sms) * (dtype == SBC_F32 ? 3 : 4);
+    const uint32_t stay = static_cast<uint32_t>(sms) * 4;
     grid = grid < stay ? grid : stay;
   }
   a.codes = static_cast<const uint8_t *>(q->codes);
