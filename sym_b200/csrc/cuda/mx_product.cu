@@ -80,7 +80,7 @@ template <int NT, bool FUSED> struct Shape {
   static constexpr int kStepA = FUSED ? NT * 128 : 0;
   static constexpr int kScaleA = FUSED ? 2 * kTileA : 0;
   static constexpr int kAcc = NT < 32 ? 32 : NT;                    // columns of the accumulator
-  static constexpr int kCols = kAcc + 64 <= 128 ? 128 : 256;        // + four buffers of 8 + 8 scale columns
+  static constexpr int kCols = kAcc + 16 * kStages <= 128 ? 128 : 256; // + 8 + 8 scale columns per stage
 };
 
 // The loading and the multiplying warp run their loops as a whole, and one
@@ -322,9 +322,9 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
       warp_wait(&full[i], i < st ? phase ^ 1 : phase, a.wait_ns);
   } else if (warp == 1) {
     // Scales go to tensor memory one stage ahead of the products that use
-    // them, so that no product waits for its own; four buffers of columns, so
-    // that a copy lies three stages of products behind the last that read its
-    // columns.
+    // them, so that no product waits for its own. Each stage has columns of its
+    // own: a stage is filled again only once the products that read it are done,
+    // so nothing still reads the columns that a copy overwrites.
     int st = 0, next = 0;
     uint32_t phase = 0;
     const auto scales = [&](uint32_t ks) {
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
       const uint32_t at = stage0 + next * S::kStage + S::kScales;
       const uint32_t at_sa =
           FUSED ? own_a + (ks1 - ks0) * S::kStepA + (ks - ks0) * S::kScaleA : at + kScaleStage;
-      const uint32_t sb = tmem + S::kAcc + (ks & 3) * 16, sa = sb + 8;
+      const uint32_t sb = tmem + S::kAcc + next * 16, sa = sb + 8;
       const uint32_t tiles = a.quads - 2 * ks < 2 ? 1 : 2;
       for (uint32_t q = 0; q < tiles; ++q) {
         copy_scales(sb + 4 * q, at + q * 512);
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
       const uint32_t left = a.k64 - 4 * ks, mmas = left < 4 ? left : 4;
       const uint32_t at = stage0 + st * S::kStage;
       const uint32_t at_a = FUSED ? own_a + (ks - ks0) * S::kStepA : at + S::kBytesB;
-      const uint32_t sb = tmem + S::kAcc + (ks & 3) * 16, sa = sb + 8;
+      const uint32_t sb = tmem + S::kAcc + st * 16, sa = sb + 8;
       const uint64_t desc_b = codes_desc(at), desc_a = codes_desc(at_a); // 32 bytes on: + 2
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i)
@@ -458,7 +458,9 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
 // them; 384 columns in two products a step measured the same within 2 %.
 // Measured with the quantisation of A: 8192 x 28672 x 8192 831 us = 4.6
 // PFLOP/s (under the power cap, SM clock near 1.35 GHz: 82 % of four times
-// cuBLAS's sustained bf16 rate), 2048 x 11008 x 4096 43.7 us = 4.2.
+// cuBLAS's sustained bf16 rate), 2048 x 11008 x 4096 43.7 us = 4.2. Given codes:
+// 8192 x 8192 x 8192 199 us = 5.5, 2048 x 4096 x 11008 35.3 us = 5.2, 2048 x 11008
+// x 4096 39.2 us = 4.7.
 // ---------------------------------------------------------------------------
 constexpr int kPairThreads = 384; // warp 0 loads, warp 1 multiplies, warps 4-11 store
 
@@ -483,10 +485,13 @@ template <int NB> struct PairShape {
   static constexpr int kScales = kBytesB + kBytesA;
   static constexpr int kStage = kScales + (1 + kGroups) * kScaleStage;
   static constexpr int kTurn = 8 * 2048; // per epilogue warp 32 columns x 32 lanes of 16-bit values
-  static constexpr int kStages = (kSmemMax - kTurn - 2048) / kStage < 8 ? (kSmemMax - kTurn - 2048) / kStage : 8;
+  static constexpr int kBufs = NB == 256 ? 1 : 2;            // accumulators of NB columns
+  static constexpr int kScaleCol = kBufs * NB;               // then, per stage, the scales' columns
+  static constexpr int kScaleCols = 8 + 8 * kGroups;
+  static constexpr int kFit = (kSmemMax - kTurn - 2048) / kStage;
+  static constexpr int kRoom = (512 - kScaleCol) / kScaleCols;
+  static constexpr int kStages = kFit < kRoom ? (kFit < 8 ? kFit : 8) : (kRoom < 8 ? kRoom : 8);
   static constexpr int kSmem = kStages * kStage + kTurn + 1024;
-  static constexpr int kBufs = NB == 256 ? 1 : 2; // accumulators in the 512 columns beside the scales
-  static constexpr int kScaleCol = kBufs * NB;
 };
 
 /// A box into this CTA's shared memory, counted on a barrier of the pair's first CTA.
@@ -624,16 +629,16 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_mx_product_pair(const __gri
   } else if (warp == 1 && rank == 0) {
     constexpr uint32_t kInstr = (1u << 7) | (1u << 10) | (static_cast<uint32_t>(NB / 8) << 17) | (1u << 23) | (2u << 27);
     // Scales go to tensor memory one stage ahead of the products that use
-    // them; four buffers of columns (see k_mx_product).
+    // them, to columns of their stage (see k_mx_product).
     int st = 0, next = 0;
-    uint32_t phase = 0, turn = 0, copied = 0, used = 0;
+    uint32_t phase = 0, turn = 0;
     bool ok = true;
     const auto scales = [&](uint32_t ks) {
       if (!warp_wait(&full[next], phase, a.wait_ns))
         return false;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t at = stage0 + next * S::kStage + S::kScales;
-      const uint32_t sb = tmem + S::kScaleCol + (copied++ & 3) * 32, sa = sb + 8;
+      const uint32_t sb = tmem + S::kScaleCol + next * S::kScaleCols, sa = sb + 8;
       const uint32_t tiles = a.quads - 2 * ks < 2 ? 1 : 2;
       for (uint32_t q = 0; q < tiles; ++q) {
         copy_scales_pair(sb + 4 * q, at + q * 512);
@@ -662,7 +667,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_mx_product_pair(const __gri
           ok = scales(ks + 1);
         const uint32_t left = a.k64 - 4 * ks, mmas = left < 4 ? left : 4;
         const uint32_t at = stage0 + st * S::kStage;
-        const uint32_t sb = tmem + S::kScaleCol + (used++ & 3) * 32, sa = sb + 8;
+        const uint32_t sb = tmem + S::kScaleCol + st * S::kScaleCols, sa = sb + 8;
         const uint64_t desc_b = codes_desc(at), desc_a = codes_desc(at + S::kBytesB); // 32 bytes on: + 2
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j)
@@ -840,7 +845,7 @@ struct Plan {
 /// less than its results take to store. The cycles are fits to measured times;
 /// over 48 shapes the choice by them loses 0.2 % against the best of the four.
 /// Measured, us, pairs of 256 / 192 / 128 / single CTAs, with given codes: 11008 x
-/// 4096 x 2048 51.2 / 46.5 / 56.3 / 109; 2048 x 11008 x 4096 38.5 / 44.0 / 55.0 /
+/// 4096 x 2048 51.2 / 48.2 / 56.3 / 109; 2048 x 11008 x 4096 38.5 / 44.0 / 55.0 /
 /// 75.6; 1003 x 8192 x 1024 10.8 / 12.0 / 13.0 / 19.9; 1003 x 1024 x 8192 16.0 /
 /// 15.4 / 14.9 / 12.3; quantised in the call, 256 x 4096 x 4096 13.0 / 11.9 / 11.3 /
 /// 12.2; 256 x 1024 x 8192 23.4 / 21.5 / 17.9 / 12.6.
