@@ -10,7 +10,7 @@
 // Measured (8192 x 8192, captured back to back; bytes of the task over time):
 //   rows, f16 26.2 us = 6.5 TB/s, f32 45.3 us = 6.7; both directions in one
 //   read, f16 40.1 us = 5.1, f32 68.5 us = 5.0 (the issue of the second
-//   direction's instructions, 66 % busy); across alone, f16 40.6 us = 4.2;
+//   direction's instructions, 66 % busy); across alone, f16 34.6 us = 4.9;
 //   back to values, f16 26.3 us = 6.5, f32 47.7 us = 6.4, transposed f16
 //   30.2 us = 5.6, f32 56 us = 5.4. [28672, 8192] to [in, out]: f16 111 us = 5.4,
 //   f32 184 us = 5.8.
@@ -138,9 +138,12 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize(const __grid_constant_
 }
 
 /// Blocks along the rows, and with ROWS along the columns too, from one read:
-/// a tile of 128 x 128 values.
+/// a tile of 128 x 128 values. 16-bit values: four blocks an SM (64 registers;
+/// across alone 34.6 us against 40.6 for 8192 x 8192). 32-bit values: as many
+/// registers as hold all of a thread's loads (116, two blocks an SM; three
+/// blocks took 79 us for both directions, two 68).
 template <int DT, bool ROWS, bool VEC>
-__global__ void __launch_bounds__(kThreads) k_mx_quantize_across(const __grid_constant__ QuantizeArgs a) {
+__global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 1 : VEC ? 4 : 3) k_mx_quantize_across(const __grid_constant__ QuantizeArgs a) {
   using T = typename Value<DT>::T;
   const int t = threadIdx.x;
   const uint32_t tr = blockIdx.x / a.tiles_c, tc = blockIdx.x - tr * a.tiles_c;
