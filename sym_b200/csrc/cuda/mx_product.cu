@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
       }
     T *y = static_cast<T *>(a.y) + (m0 + c) * a.n + n;
     if (a.y_vec && n < a.n) { // n is a multiple of 4, and so is a.n
-      T out[4];
+      alignas(16) T out[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         out[i] = Value<DT>::down(v[i]);

@@ -644,3 +644,15 @@ def test_copies_of_a_matrix_own_their_memory():
     torch.cuda.empty_cache()
     for c in copies:
         assert torch.equal(mx.linear(x, c), want)
+
+
+@pytest.mark.parametrize("rows,cols", [(128, 40), (40, 128), (256, 129), (128, 1)])
+def test_absent_blocks_have_scale_zero(rows, cols):
+    """The bytes of a row's last scale tile that belong to no block are 0, in
+    either direction: a product may read them beside zero codes."""
+    x = tensor((rows, cols), torch.bfloat16, 73).abs() + 1  # no block has the scale byte 0
+    for q in (mx.quantize(x), mx.quantize(x, along=0), *mx.quantize_both(x)):
+        r, c = q.shape
+        blocks, quads = O.blocks_of(c), -(-c // 128)
+        tiles = q.scales.view(-(-r // 128), quads, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(-1, quads * 4)[:r]
+        assert (tiles[:, :blocks] > 0).all() and (tiles[:, blocks:] == 0).all()
