@@ -1,5 +1,5 @@
 """The microscaled formats in numpy with 64-bit arithmetic, from their
-definition; the checker of tests/test_microscale*.py."""
+definition; the oracle of tests/test_microscale*.py."""
 import numpy as np
 
 E2M1 = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])

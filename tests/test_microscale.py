@@ -1,4 +1,4 @@
-"""Microscaled matrices without a GPU: the formats' checker against hand-made
+"""Microscaled matrices without a GPU: the formats' oracle against hand-made
 values, the scale layout, and what the calls refuse."""
 import ctypes
 import math
@@ -12,7 +12,7 @@ from sym_b200 import _native
 from sym_b200 import microscale as mx
 
 
-def test_checker_on_hand_made_blocks():
+def test_oracle_on_hand_made_blocks():
     x = np.zeros((1, 64))
     # largest 7 = 1.75 2^2: scale 2^0; ties to even codes, 7 saturates
     x[0, :12] = [7, 5, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, -5, -0.25, 0.26, 4.9]
