@@ -91,7 +91,10 @@ template <int NT, bool FUSED> struct Shape {
 // to 128 that the product needs.
 #define SBC_ELECTED(instruction) "{\n .reg .pred one;\n elect.sync _|one, 0xffffffff;\n @one " instruction "\n}"
 
-/// A bounded wait of the whole warp.
+/// A bounded wait of the whole warp, with one answer for all lanes: a warp
+/// whose lanes each went by their own clock could leave a loop in parts, and
+/// the tensor-memory loads, stmatrix and elections behind these waits need
+/// every lane. The only wait of these kernels, in every warp.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, uint64_t limit_ns) {
   return __all_sync(~0u, mbar_wait_often(bar, parity, limit_ns));
 }
@@ -375,7 +378,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
     const int quarter = warp & 3; // the lanes of tensor memory that this warp may read
     const int row = quarter * 32 + lane;
     const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    if (!mbar_wait_often(&ready, 0, a.wait_ns))
+    if (!warp_wait(&ready, 0, a.wait_ns))
       *a.fault = 2;
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     // The part's sums as [cols][128] in the stages, all of which have been read.
@@ -691,7 +694,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_mx_product_pair(const __gri
       const uint32_t buf = turn % S::kBufs, use = turn / S::kBufs;
       uint32_t tb, ta;
       pair_tile(a, i, tb, ta);
-      if (!mbar_wait_often(&ready[buf], use & 1, a.wait_ns)) {
+      if (!warp_wait(&ready[buf], use & 1, a.wait_ns)) {
         *a.fault = 2;
         break;
       }
