@@ -169,6 +169,20 @@ void sbc_set_wait_limit_ns(uint64_t ns);
  * `wait_limit_ns`, sbc_mx_take_fault reports it, and the launch after it is
  * normal again. 0 disarms. */
 void sbc_test_withhold_mx(uint64_t wait_limit_ns);
+/* sbc_test_mx_plan: what the product of these sizes would take on a device of
+ * `sms` SMs, by host arithmetic alone: the rows of a that a pair of SMs takes
+ * per tile (0: single CTAs), the rows that a single CTA takes, the CTAs that share
+ * a tile along k, whether a is quantised in the kernel, and the tiles that a pair
+ * (a cluster of single CTAs: 1) works through. 0, or SBC_EINVAL for sizes that
+ * are refused. */
+typedef struct {
+  int32_t pair;
+  int32_t single;
+  int32_t split;
+  int32_t fused;
+  int32_t turns;
+} sbc_mx_choice;
+int sbc_test_mx_plan(int64_t m, int64_t n, int64_t k, int32_t sms, sbc_mx_choice *out);
 int sbc_test_fault_mode(int mode);
 void sbc_test_withhold_tile(uint32_t job, uint64_t wait_limit_ns);
 

@@ -43,6 +43,10 @@ class SbGroupEntry(ctypes.Structure):
     _fields_ = [("plan", ctypes.c_void_p), ("source", SbView), ("destination", SbView), ("direction", ctypes.c_int32)]
 
 
+class SbcMxChoice(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_int32) for name in ("pair", "single", "split", "fused", "turns")]
+
+
 class SbMx(ctypes.Structure):
     _fields_ = [("codes", ctypes.c_uint64), ("scales", ctypes.c_uint64), ("rows", ctypes.c_int64),
                 ("cols", ctypes.c_int64), ("format", ctypes.c_int32), ("device", ctypes.c_int32)]
@@ -138,7 +142,7 @@ def cuda_layer():
     """The thin CUDA layer (libsb_cuda.so, include/sb_cuda.h), loaded by the
     runtime library; for its wait-limit setting and the test hooks that
     inject failures (``sbc_test_fault_mode``, ``sbc_test_withhold_tile``,
-    ``sbc_test_withhold_mx``)."""
+    ``sbc_test_withhold_mx``) or tell the kernel choice (``sbc_test_mx_plan``)."""
     global _cuda
     if _cuda is not None:
         return _cuda
@@ -150,6 +154,9 @@ def cuda_layer():
     L.sbc_test_withhold_tile.argtypes = [ctypes.c_uint32, ctypes.c_uint64]
     L.sbc_test_withhold_mx.restype = None
     L.sbc_test_withhold_mx.argtypes = [ctypes.c_uint64]
+    L.sbc_test_mx_plan.restype = ctypes.c_int
+    L.sbc_test_mx_plan.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
+                                   ctypes.POINTER(SbcMxChoice)]
     L.sbc_set_wait_limit_ns.restype = None
     L.sbc_set_wait_limit_ns.argtypes = [ctypes.c_uint64]
     L.sbc_wait_launch_count.restype = ctypes.c_uint64

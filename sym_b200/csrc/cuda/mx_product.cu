@@ -1052,6 +1052,15 @@ extern "C" {
 
 void sbc_test_withhold_mx(uint64_t wait_limit_ns) { g_withhold.store(wait_limit_ns, std::memory_order_relaxed); }
 
+int sbc_test_mx_plan(int64_t m, int64_t n, int64_t k, int32_t sms, sbc_mx_choice *out) {
+  Plan p;
+  if (!out || m <= 0 || n <= 0 || k <= 0 || !plan_of(m, n, k, sms, &p))
+    return SBC_EINVAL;
+  const int64_t pairs = sms / 2, tiles = p.pair ? (m + p.pair - 1) / p.pair * ((n + 255) / 256) : 1;
+  *out = sbc_mx_choice{p.pair, p.nt, p.split, p.fused, static_cast<int32_t>(p.pair ? (tiles + pairs - 1) / pairs : 1)};
+  return 0;
+}
+
 int sbc_mx_take_fault(void) {
   int32_t *w = fault_word();
   if (!w)
