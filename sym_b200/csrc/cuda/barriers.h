@@ -1,5 +1,5 @@
-// sym_b200 -- shared-memory barriers with bounded waits, and the tensor map
-// encoder: what every kernel that is fed by asynchronous copies uses.
+// sym_b200 -- shared-memory barriers with bounded waits, and the encoding of
+// tensor maps: what every kernel that is fed by asynchronous copies uses.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -32,8 +32,11 @@ template <auto KERNEL> cudaError_t allow_shared(int bytes) {
   return e;
 }
 
-/// cuTensorMapEncodeTiled of the loaded driver, or NULL.
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
+/// A tiled tensor map (unit element strides, what lies past the end reads as
+/// 0); false where the driver lacks or refuses it. May be a thread's first CUDA
+/// call.
+bool encode_tiled(CUtensorMap *map, CUtensorMapDataType type, uint32_t rank, const void *base, const cuuint64_t *dims,
+                  const cuuint64_t *strides, const cuuint32_t *box, CUtensorMapSwizzle swizzle);
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -894,16 +894,10 @@ bool plan_of(int64_t m, int64_t n, int64_t k, int sms, Plan *p) {
 /// Codes [rows, pitch] as boxes of `box_rows` rows x 128 bytes; what lies past
 /// the end reads as zero codes.
 bool encode_codes(CUtensorMap *map, const void *base, int64_t rows, int64_t pitch, int box_rows) {
-  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
-  if (!enc)
-    return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
   const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t estr[2] = {1, 1};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int DT, int XT, int NT, bool FUSED> int launch(const ProductArgs &a, const Plan &p, cudaStream_t s) {
@@ -938,16 +932,10 @@ template <int DT, int XT, int NT, bool FUSED> int launch(const ProductArgs &a, c
 /// Scale tiles of a matrix [rows, cols] as rows of 512 bytes, boxes of two; what
 /// lies past the end reads as 0.
 bool encode_scales(CUtensorMap *map, const void *base, int64_t rows, int64_t quads) {
-  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
-  if (!enc)
-    return false;
   const cuuint64_t dims[2] = {128, static_cast<cuuint64_t>((rows + 127) / 128 * quads)};
   const cuuint64_t strides[1] = {512};
   const cuuint32_t box[2] = {128, 2};
-  const cuuint32_t estr[2] = {1, 1};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void *>(base), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 template <int DT, int NB> int launch_pair(const ProductArgs &a, const sbc_mx *qa, const sbc_mx *qb, int sms, cudaStream_t s) {

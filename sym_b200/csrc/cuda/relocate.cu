@@ -2141,8 +2141,7 @@ uint32_t tma_group_log2() {
 /// description (the caller then uses a SIMT tile kernel).
 bool encode_rows3d(CUtensorMap *map, const void *base, int ws, int64_t cols, int64_t rows, int64_t pitch, int gr,
                    int tile_rows = 64) {
-  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
-  if (!enc || reinterpret_cast<uintptr_t>(base) % 16 || pitch % 16 || rows % gr || (ws != 1 && ws != 4) ||
+  if (reinterpret_cast<uintptr_t>(base) % 16 || pitch % 16 || rows % gr || (ws != 1 && ws != 4) ||
       (gr != 4 && gr != 8) || (tile_rows != 64 && tile_rows != 128))
     return false;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows / gr),
@@ -2150,12 +2149,8 @@ bool encode_rows3d(CUtensorMap *map, const void *base, int ws, int64_t cols, int
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch * gr), static_cast<cuuint64_t>(pitch)};
   const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / ws), static_cast<cuuint32_t>(tile_rows / gr),
                              static_cast<cuuint32_t>(gr)};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = enc(map, ws == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT32, 3,
-                         const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
+  return encode_tiled(map, ws == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, base, dims, strides,
+                      box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int WS, int WD, int CH> struct TileLaunch {
@@ -2458,7 +2453,8 @@ void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 void count_wait_launch() { g_wait_launches.fetch_add(1, std::memory_order_relaxed); }
 uint64_t wait_limit_ns() { return g_wait_ns.load(std::memory_order_relaxed); }
 
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+bool encode_tiled(CUtensorMap *map, CUtensorMapDataType type, uint32_t rank, const void *base, const cuuint64_t *dims,
+                  const cuuint64_t *strides, const cuuint32_t *box, CUtensorMapSwizzle swizzle) {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -2470,7 +2466,20 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     else
       cudaGetLastError();
   });
-  return fn;
+  if (!fn)
+    return false;
+  const cuuint32_t unit[5] = {1, 1, 1, 1, 1};
+  const auto encode = [&] {
+    return fn(map, type, rank, const_cast<void *>(base), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (encode())
+    return true;
+  // The driver wants a context in the calling thread. Runtime calls bind the
+  // current device's when they need it; a thread that has made none yet (a
+  // worker's or a backward pass's first product) gets it here.
+  int device = 0;
+  return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && encode();
 }
 
 } // namespace sbc
