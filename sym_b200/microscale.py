@@ -27,6 +27,12 @@ torch's caching allocator only and can be captured into CUDA graphs (a backward
 pass, as torch asks, only while no eager graph of the same leaves is alive).
 They have no CPU execution. Wrong arguments raise ``ValueError`` or ``TypeError``; failures of the
 native layer raise ``pyreloc.TransferError``.
+
+Derivatives are those of reverse mode, once; codes carry none. Forward-mode
+tangents, ``vmap`` and second derivatives are refused. The kernels get addresses, which
+a recorder of torch operations cannot see: ``make_fx`` is refused with
+``NotImplementedError``, and so is ``torch.jit.trace`` but for ``linear`` and
+``silu_mul``, which it records as autograd functions.
 """
 from __future__ import annotations
 
@@ -35,6 +41,7 @@ import threading
 from functools import lru_cache
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _native
 from .pyreloc import _raise_transfer
@@ -62,6 +69,32 @@ def _check(rc):
 def _stream(index):
     """The current stream (a cudaStream_t) of a device."""
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+_modes = torch._C._len_torch_dispatch_stack
+_key_included = torch._C._dispatch_tls_is_dispatch_key_included
+_PRE_DISPATCH = torch._C.DispatchKey.PreDispatch
+_jit_tracing = torch._C._is_tracing
+
+
+def _traceable(call, jit=False):
+    """Refuses a call whose result a recorder would keep as the allocation alone:
+    under make_fx, and where the call is no autograd function (``jit``) under
+    torch.jit.trace."""
+    if _modes() or _key_included(_PRE_DISPATCH):
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+
+        if get_proxy_mode() is not None:
+            raise NotImplementedError(f"{call} cannot be recorded by make_fx: its kernels take addresses")
+    if jit and _jit_tracing():
+        raise NotImplementedError(f"{call} cannot be recorded by torch.jit.trace: its kernels take addresses")
+
+
+def _no_tangents(call, *tensors):
+    """Refuses inputs with forward-mode tangents, which would be lost."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{call} has no forward-mode derivative")
 
 
 _library = None
@@ -178,9 +211,8 @@ class MxTensor:
         return f"MxTensor({list(self.shape)}, {self.format}, {self.device})"
 
 
-def _matrix(x):
-    """x as a matrix whose columns are adjacent: (tensor, rows, cols, row stride)."""
-    cols = x.shape[-1]
+def _matrix(x, cols):
+    """x [..., cols] as a matrix whose columns are adjacent: (tensor, rows, cols, row stride)."""
     if x.is_contiguous():
         return x, x.numel() // cols, cols, cols
     if x.dim() != 2:
@@ -191,16 +223,18 @@ def _matrix(x):
     return x, rows, cols, x.stride(0) if rows > 1 else cols
 
 
-def _values(x, name, least=1):
+def _values(x, name):
+    """The shape of a tensor of values, once it is one that the kernels take."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} is a tensor")
     if x.dtype not in _DTYPES:
         raise TypeError(f"{name} is float32, float16 or bfloat16")
     if not x.is_cuda:
         raise ValueError(f"{name} is on {x.device}: microscaled operators run on CUDA devices")
-    if x.dim() < least or x.shape[-1] == 0:
-        raise ValueError(f"{name} needs {'rows and columns' if least == 2 else 'at least one column'}")
-    return x
+    shape = x.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{name} needs at least one column")
+    return shape
 
 
 def _mx(q, name, format=None):
@@ -220,8 +254,8 @@ def _result(dtype, default):
     return dtype
 
 
-def _quantize(x, format, along, across):
-    x, rows, cols, stride = _matrix(x)
+def _quantize(x, cols, format, along, across):
+    x, rows, cols, stride = _matrix(x, cols)
     q = MxTensor._empty(x, rows, cols, format) if along else None
     qt = MxTensor._empty(x, cols, rows) if across else None
     if rows:
@@ -265,7 +299,7 @@ def _differentiable_once(backward):
 
 
 def _quantize_into(x, along, across):
-    x, rows, cols, stride = _matrix(x)
+    x, rows, cols, stride = _matrix(x, x.shape[-1])
     _check(_lib().sb_mx_quantize(x.data_ptr(), _DTYPES[x.dtype], rows, cols, stride, along, across,
                                  _stream(x.get_device()), _scratch.ref))
 
@@ -280,42 +314,45 @@ def quantize(x, format="mxfp4", *, along=-1):
     along the last axis (leading axes are flattened), or for a matrix with
     ``along=0`` to the mxfp4 form of its transpose, whose blocks run along
     the first axis."""
-    _values(x, "x")
+    _traceable("quantize", jit=True)
+    shape = _values(x, "x")
     if format not in FORMATS:
         raise ValueError(f"format must be one of {sorted(FORMATS)}")
     if along not in (0, -1):
         raise ValueError("along must be -1 or 0")
-    x = x.detach()
     if along == 0:
-        if x.dim() != 2 or x.shape[0] == 0:
+        if len(shape) != 2 or shape[0] == 0:
             raise ValueError("along=0 takes a matrix with at least one row")
         if format != "mxfp4":
             raise ValueError("along=0 is defined for mxfp4")
-    if x.dim() == 2 and format == "mxfp4" and x.shape[0] > 1 and x.shape[1] > 1 and x.stride(0) == 1 != x.stride(1):
+    if len(shape) == 2 and format == "mxfp4" and shape[0] > 1 and shape[1] > 1 and x.stride(0) == 1 != x.stride(1):
         # a transposed view: the other direction of the matrix behind it
-        return _quantize(x.t(), format, along == 0, along != 0)[0 if along == 0 else 1]
-    q, qt = _quantize(x, format, along != 0, along == 0)
+        return _quantize(x.t(), shape[0], format, along == 0, along != 0)[0 if along == 0 else 1]
+    q, qt = _quantize(x, shape[-1], format, along != 0, along == 0)
     return q if qt is None else qt
 
 
 def quantize_both(x):
     """A matrix's two mxfp4 forms with one read of it: ``(quantize(x),
     quantize(x, along=0))``, what a training step's products take."""
-    if _values(x, "x").dim() != 2 or x.shape[0] == 0:
+    _traceable("quantize_both", jit=True)
+    shape = _values(x, "x")
+    if len(shape) != 2 or shape[0] == 0:
         raise ValueError("quantize_both takes a matrix with at least one row")
-    return _quantize(x.detach(), "mxfp4", True, True)
+    return _quantize(x, shape[1], "mxfp4", True, True)
 
 
 def dequantize(q, dtype=torch.float16, *, transpose=False):
     """The values of an ``MxTensor``, each rounded once to ``dtype``: ``[rows,
     cols]``, or ``[cols, rows]`` with ``transpose`` (mxfp4), the layout that a
     product ``x @ w`` takes."""
+    _traceable("dequantize", jit=True)
     _mx(q, "q")
     dtype = _result(dtype, None)
     if transpose and q.format != "mxfp4":
         raise ValueError("transpose is defined for mxfp4")
     rows, cols = q.shape
-    out = torch.empty((cols, rows) if transpose else (rows, cols), dtype=dtype, device=q.device)
+    out = q._codes.new_empty((cols, rows) if transpose else (rows, cols), dtype=dtype)
     if rows:
         _check(_lib().sb_mx_dequantize(q.native, out.data_ptr(), _DTYPES[dtype], int(transpose),
                                        _stream(q.get_device()), _scratch.ref))
@@ -332,6 +369,7 @@ def _linear_workspace(m, n, k, device):
 def matmul(a, b, *, dtype=torch.bfloat16):
     """``a [m, k]`` times the transpose of ``b [n, k]``, both mxfp4, accumulated in
     32 bits and rounded once to ``dtype``."""
+    _traceable("matmul", jit=True)
     _mx(a, "a", "mxfp4"), _mx(b, "b", "mxfp4")
     dtype = _result(dtype, None)
     if a.device != b.device:
@@ -343,10 +381,10 @@ def matmul(a, b, *, dtype=torch.bfloat16):
     return _matmul_into(a.native, b.native, y) if m and n else y
 
 
-def _linear(x, w, dtype):
-    shape = x.shape
-    x, m, k, stride = _matrix(x)
-    n = w.shape[0]
+def _linear(x, w, dtype, shape):
+    """x [shape] times the transpose of w."""
+    n, k = w._shape
+    x, m, _, stride = _matrix(x, k)
     y = x.new_empty((*shape[:-1], n), dtype=dtype)
     if m and n:
         index = x.get_device()
@@ -362,14 +400,18 @@ class _FrozenLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, wt, dtype):
-        ctx.save_for_backward(wt.codes, wt.scales)
-        ctx.shape, ctx.dtype = wt.shape, x.dtype
-        return _linear(x, w, dtype)
+        ctx.shape = None
+        if wt is not None:
+            ctx.save_for_backward(wt.codes, wt.scales)
+            ctx.shape, ctx.dtype = wt.shape, x.dtype
+        return _linear(x, w, dtype, x.shape)
 
     @staticmethod
     @_differentiable_once
     def backward(ctx, dy):
-        return _linear(dy, MxTensor(*ctx.saved_tensors, ctx.shape), ctx.dtype), None, None, None
+        if ctx.shape is None:
+            raise ValueError("x needs a gradient: linear was recorded without weight_t")
+        return _linear(dy, MxTensor(*ctx.saved_tensors, ctx.shape), ctx.dtype, dy.shape), None, None, None
 
 
 class _TrainLinear(torch.autograd.Function):
@@ -427,23 +469,33 @@ def linear(x, weight, weight_t=None, *, dtype=None):
 
     ``weight`` a float tensor: training; x, weight and dy are quantised along the
     axis that each product sums over, and the backward pass gives dx and dw."""
-    _values(x, "x")
+    _traceable("linear")
+    if _forward_ad._current_level >= 0:
+        _no_tangents("linear", x, weight)
+    shape = _values(x, "x")
     dtype = _result(dtype, x.dtype)
-    if type(weight) is MxTensor:
+    frozen = type(weight) is MxTensor
+    if frozen:
         _mx(weight, "weight", "mxfp4")
+        n, k = weight._shape
     elif weight_t is not None:
         raise ValueError("weight_t goes with an MxTensor weight")
-    elif _values(weight, "weight").dim() != 2:
-        raise ValueError("weight is a matrix [n, k]")
+    else:
+        extents = _values(weight, "weight")
+        if len(extents) != 2:
+            raise ValueError("weight is a matrix [n, k]")
+        n, k = extents
     if weight.get_device() != x.get_device():
         raise ValueError("x and weight live on different devices")
-    n, k = weight.shape
-    if x.shape[-1] != k:
-        raise ValueError(f"x [..., k] and weight [n, k] need the same k: got {x.shape[-1]} and {k}")
-    if type(weight) is MxTensor:
-        if not (x.requires_grad and torch.is_grad_enabled()):
-            return _linear(x, weight, dtype)
+    if shape[-1] != k:
+        raise ValueError(f"x [..., k] and weight [n, k] need the same k: got {shape[-1]} and {k}")
+    if frozen:
+        needs = x.requires_grad and torch.is_grad_enabled()
+        if not (needs or _jit_tracing()):
+            return _linear(x, weight, dtype, shape)
         if weight_t is None:
+            if not needs:
+                return _FrozenLinear.apply(x, weight, None, dtype)
             raise ValueError("x needs a gradient: pass weight_t, the mxfp4 form of the weight's transpose")
         if _mx(weight_t, "weight_t", "mxfp4").shape != (k, n) or weight_t.device != x.device:
             raise ValueError(f"weight_t is [{k}, {n}] on {x.device}")
@@ -473,7 +525,7 @@ class _SiluMul(torch.autograd.Function):
         dup = None if ctx.packed else dh.new_empty(ctx.shape)
         if gate.rows:
             cols, dtype = gate.cols, dh.dtype
-            dh, _, _, stride = _matrix(dh)
+            dh, _, _, stride = _matrix(dh, cols)
             out = 2 * cols if ctx.packed else cols
             at = dgate.data_ptr() + cols * dh.element_size() if ctx.packed else dup.data_ptr()
             _check(_lib().sb_silu_mul_backward(dh.data_ptr(), stride, _DTYPES[dtype], gate, up, dgate.data_ptr(), out,
@@ -482,9 +534,10 @@ class _SiluMul(torch.autograd.Function):
 
 
 def _silu_mul(gate, up, kept_gate=None, kept_up=None):
-    h = gate.new_empty(gate.shape)
-    gate, rows, cols, gate_stride = _matrix(gate)
-    up, _, _, up_stride = _matrix(up)
+    shape = gate.shape
+    h = gate.new_empty(shape)
+    gate, rows, cols, gate_stride = _matrix(gate, shape[-1])
+    up, _, _, up_stride = _matrix(up, cols)
     if rows:
         index = gate.get_device()
         _check(_lib().sb_silu_mul(gate.data_ptr(), gate_stride, up.data_ptr(), up_stride, _DTYPES[gate.dtype], rows,
@@ -500,14 +553,17 @@ def silu_mul(gate, up=None):
     per value, step at most 2^-6 of the block's largest magnitude) instead of
     as they are, and the backward pass computes both gradients from the copies.
     The result itself is computed from the inputs."""
-    _values(gate, "gate")
+    _traceable("silu_mul")
+    if _forward_ad._current_level >= 0:
+        _no_tangents("silu_mul", gate, up)
+    shape = _values(gate, "gate")
     if up is None:
-        if gate.shape[-1] % 2:
+        if shape[-1] % 2:
             raise ValueError("gate and up in one tensor need an even last axis")
     else:
-        _values(up, "up")
-        if up.shape != gate.shape or up.dtype != gate.dtype or up.device != gate.device:
+        if _values(up, "up") != shape or up.dtype != gate.dtype or up.device != gate.device:
             raise ValueError("gate and up have the same shape, type and device")
-    if torch.is_grad_enabled() and (gate.requires_grad or (up is not None and up.requires_grad)):
+    needs = torch.is_grad_enabled() and (gate.requires_grad or (up is not None and up.requires_grad))
+    if needs or _jit_tracing():
         return _SiluMul.apply(gate, up)
-    return _silu_mul(*(gate.detach().chunk(2, -1) if up is None else (gate.detach(), up.detach())))
+    return _silu_mul(*gate.chunk(2, -1)) if up is None else _silu_mul(gate, up)

@@ -1,0 +1,100 @@
+"""Microscaled calls under torch's other derivatives and its recorders: what
+cannot be right is refused, what is recorded gives the call's result.
+
+The CPU tests need no CUDA tensor: such a call is refused before its tensors
+are looked at, where it used to go on to the tensors' addresses."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+from torch.fx.experimental.proxy_tensor import make_fx
+
+from sym_b200 import microscale as mx
+
+
+def host_matrix(rows=4, cols=64):
+    return mx.MxTensor(torch.zeros(rows, cols // 2, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8), (rows, cols))
+
+
+def test_forward_mode_tangents_are_refused():
+    x, w, q = torch.ones(2, 64), torch.ones(4, 64), host_matrix()
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda: mx.linear(d, q), lambda: mx.linear(d, q, q), lambda: mx.linear(d, w),
+                     lambda: mx.linear(x, fw.make_dual(w, w)), lambda: mx.silu_mul(d), lambda: mx.silu_mul(x, d)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(ValueError, match="CUDA"):
+            mx.linear(x, q)  # without a tangent it is an ordinary call
+
+
+@pytest.mark.parametrize("pre_dispatch", (False, True))
+def test_make_fx_is_refused(pre_dispatch):
+    x, q = torch.ones(2, 64), host_matrix()
+    for call in (lambda x: mx.linear(x, q), lambda x: mx.linear(x, x), lambda x: mx.silu_mul(x),
+                 lambda x: mx.quantize(x).codes, lambda x: mx.quantize_both(x)[0].codes, lambda x: mx.dequantize(q),
+                 lambda x: mx.matmul(q, q)):
+        with pytest.raises(NotImplementedError, match="make_fx"):
+            make_fx(call, pre_dispatch=pre_dispatch)(x)
+
+
+def test_tracing_of_calls_that_are_no_autograd_functions_is_refused():
+    x, q = torch.ones(2, 64), host_matrix()
+    for call in (lambda x: mx.quantize(x).codes, lambda x: mx.quantize_both(x)[0].codes, lambda x: mx.dequantize(q),
+                 lambda x: mx.matmul(q, q)):
+        with pytest.raises(NotImplementedError, match="jit"):
+            torch.jit.trace(call, (x,), check_trace=False)
+
+
+def test_other_dispatch_modes_are_no_recorders():
+    from torch.utils.flop_counter import FlopCounterMode
+
+    with FlopCounterMode(display=False), pytest.raises(ValueError, match="CUDA"):
+        mx.silu_mul(torch.ones(2, 64))
+
+
+def tensor(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+@pytest.mark.gpu
+def test_traces_give_the_calls_results():
+    x, w = tensor(5, 64), tensor(96, 64, seed=1)
+    q, qt = mx.quantize_both(w)
+    other = tensor(5, 64, seed=2)
+    for call in (lambda x: mx.linear(x, q) + 1, lambda x: mx.linear(x, q, qt) + 1, lambda x: mx.silu_mul(x) * 2,
+                 lambda x: mx.silu_mul(x, x + 1), lambda x: mx.linear(x, w), lambda x: mx.silu_mul(mx.linear(x, q))):
+        traced = torch.jit.trace(call, (x,), check_trace=False)
+        for _ in range(3):  # the first runs of a trace are its profiling ones
+            torch.empty(1 << 20, device="cuda").fill_(float("nan"))  # what an allocation alone would hold
+            assert torch.equal(traced(other), call(other))
+    xg = x.clone().requires_grad_()
+    traced = torch.jit.trace(lambda x: mx.linear(x, q, qt), (xg,), check_trace=False)
+    dy = tensor(5, 96, seed=3)
+    want, = torch.autograd.grad(mx.linear(xg, q, qt), xg, dy)
+    got, = torch.autograd.grad(traced(xg), xg, dy)
+    assert torch.equal(got, want)
+    without = torch.jit.trace(lambda x: mx.linear(x, q), (x,), check_trace=False)
+    with pytest.raises(Exception, match="weight_t"):
+        torch.autograd.grad(without(xg).sum(), xg)
+
+
+@pytest.mark.gpu
+def test_forward_mode_and_transforms_on_the_gpu():
+    x, w = tensor(5, 64), tensor(96, 64, seed=1)
+    q = mx.quantize(w)
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda: mx.linear(d, q), lambda: mx.linear(d, w), lambda: mx.silu_mul(d)):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(mx.linear(x, q), mx.linear(fw.unpack_dual(d).primal, q))
+    for call in (lambda x: mx.linear(x, q), lambda x: mx.silu_mul(x), lambda x: mx.linear(x, w)):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(call, (x,), (x,))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(x.view(5, 1, 64))
+        for mode in ("real", "fake", "symbolic"):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                make_fx(call, tracing_mode=mode)(x)
