@@ -32,7 +32,8 @@ Derivatives are those of reverse mode, once; codes carry none. Forward-mode
 tangents, ``vmap`` and second derivatives are refused. The kernels get addresses, which
 a recorder of torch operations cannot see: ``make_fx`` is refused with
 ``NotImplementedError``, and so is ``torch.jit.trace`` but for ``linear`` and
-``silu_mul``, which it records as autograd functions.
+``silu_mul``, which it records as autograd functions; ``torch.compile`` runs the
+calls as they are, between its graphs.
 """
 from __future__ import annotations
 
@@ -75,6 +76,14 @@ _modes = torch._C._len_torch_dispatch_stack
 _key_included = torch._C._dispatch_tls_is_dispatch_key_included
 _PRE_DISPATCH = torch._C.DispatchKey.PreDispatch
 _jit_tracing = torch._C._is_tracing
+_compiling = torch.compiler.is_dynamo_compiling
+
+
+def _uncompiled(call, *args, **kwargs):
+    """A call as torch.compile runs it: as it is, between two graphs. Its frames
+    are not taken apart, which would free tensors whose addresses a kernel is
+    still to get."""
+    return torch.compiler.disable(call)(*args, **kwargs)
 
 
 def _traceable(call, jit=False):
@@ -293,6 +302,8 @@ def _differentiable_once(backward):
     guarded = torch.autograd.function.once_differentiable(backward)
 
     def run(ctx, *grads):
+        if _compiling():
+            return _uncompiled(run, ctx, *grads)
         return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
     return run
@@ -314,6 +325,8 @@ def quantize(x, format="mxfp4", *, along=-1):
     along the last axis (leading axes are flattened), or for a matrix with
     ``along=0`` to the mxfp4 form of its transpose, whose blocks run along
     the first axis."""
+    if _compiling():
+        return _uncompiled(quantize, x, format, along=along)
     _traceable("quantize", jit=True)
     shape = _values(x, "x")
     if format not in FORMATS:
@@ -335,6 +348,8 @@ def quantize(x, format="mxfp4", *, along=-1):
 def quantize_both(x):
     """A matrix's two mxfp4 forms with one read of it: ``(quantize(x),
     quantize(x, along=0))``, what a training step's products take."""
+    if _compiling():
+        return _uncompiled(quantize_both, x)
     _traceable("quantize_both", jit=True)
     shape = _values(x, "x")
     if len(shape) != 2 or shape[0] == 0:
@@ -346,6 +361,8 @@ def dequantize(q, dtype=torch.float16, *, transpose=False):
     """The values of an ``MxTensor``, each rounded once to ``dtype``: ``[rows,
     cols]``, or ``[cols, rows]`` with ``transpose`` (mxfp4), the layout that a
     product ``x @ w`` takes."""
+    if _compiling():
+        return _uncompiled(dequantize, q, dtype, transpose=transpose)
     _traceable("dequantize", jit=True)
     _mx(q, "q")
     dtype = _result(dtype, None)
@@ -369,6 +386,8 @@ def _linear_workspace(m, n, k, device):
 def matmul(a, b, *, dtype=torch.bfloat16):
     """``a [m, k]`` times the transpose of ``b [n, k]``, both mxfp4, accumulated in
     32 bits and rounded once to ``dtype``."""
+    if _compiling():
+        return _uncompiled(matmul, a, b, dtype=dtype)
     _traceable("matmul", jit=True)
     _mx(a, "a", "mxfp4"), _mx(b, "b", "mxfp4")
     dtype = _result(dtype, None)
@@ -469,6 +488,8 @@ def linear(x, weight, weight_t=None, *, dtype=None):
 
     ``weight`` a float tensor: training; x, weight and dy are quantised along the
     axis that each product sums over, and the backward pass gives dx and dw."""
+    if _compiling():
+        return _uncompiled(linear, x, weight, weight_t, dtype=dtype)
     _traceable("linear")
     if _forward_ad._current_level >= 0:
         _no_tangents("linear", x, weight)
@@ -553,6 +574,8 @@ def silu_mul(gate, up=None):
     per value, step at most 2^-6 of the block's largest magnitude) instead of
     as they are, and the backward pass computes both gradients from the copies.
     The result itself is computed from the inputs."""
+    if _compiling():
+        return _uncompiled(silu_mul, gate, up)
     _traceable("silu_mul")
     if _forward_ad._current_level >= 0:
         _no_tangents("silu_mul", gate, up)

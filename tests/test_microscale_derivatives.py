@@ -98,3 +98,33 @@ def test_forward_mode_and_transforms_on_the_gpu():
         for mode in ("real", "fake", "symbolic"):
             with pytest.raises((RuntimeError, NotImplementedError)):
                 make_fx(call, tracing_mode=mode)(x)
+
+
+@pytest.mark.gpu
+def test_compiled_regions_run_the_calls_between_their_graphs():
+    x, w = tensor(5, 64), tensor(96, 64, seed=1)
+    q, qt = mx.quantize_both(w)
+
+    def layer(x, w):
+        a = mx.linear(x * 2, w) + 1
+        b = mx.linear(torch.sin(x), q, qt)
+        return mx.silu_mul(a, b).sum()
+
+    xs = [x.clone().requires_grad_() for _ in range(2)]
+    ws = [w.clone().requires_grad_() for _ in range(2)]
+    compiled = torch.compile(layer, backend="eager")
+    for _ in range(2):
+        want = torch.autograd.grad(layer(xs[0], ws[0]), (xs[0], ws[0]))
+        got = torch.autograd.grad(compiled(xs[1], ws[1]), (xs[1], ws[1]))
+        assert torch.equal(compiled(xs[1], ws[1]), layer(xs[0], ws[0]))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad():
+        for call in (lambda x: mx.linear(x, q) * 2, lambda x: mx.quantize(x).codes.clone(),
+                     lambda x: mx.quantize_both(x + 1)[1].codes + 1,
+                     lambda x: mx.dequantize(mx.quantize(x * 2), torch.float32) + 1,
+                     lambda x: mx.matmul(mx.quantize(x, along=0), mx.quantize(x + 1, along=0)) * 2,
+                     lambda x: mx.linear(x, mx.MxTensor(q.codes.clone(), q.scales.clone(), (96, 64))) + 1,
+                     lambda x: mx.linear(x, mx.MxTensor.from_rows(q.codes.clone(), q.row_scales(), 64)) + 1,
+                     lambda x: mx.linear(x, q.to("cpu").to("cuda")) + 1):
+            assert torch.equal(torch.compile(call, backend="eager")(x), call(x))
+            torch._dynamo.reset()
