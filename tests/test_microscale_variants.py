@@ -21,9 +21,9 @@ SMS = 148
 PAIRS = [(1003, 4101, 520), (1347, 9703, 66), (2737, 8767, 65), (300, 9001, 520), (777, 11008, 512),
          (1110, 11371, 67), (1468, 9525, 1000), (1822, 11893, 67), (163, 768, 68), (831, 7618, 520),
          (1541, 8364, 520)]
-SINGLES = [(1, 512, 2048), (3, 700, 500), (8, 2000, 4096), (2, 5000, 200), (7, 19500, 500), (13, 20000, 100), (16, 900, 4096),
-           (32, 300, 1000), (30, 19000, 64), (64, 1000, 4096), (50, 19001, 96), (128, 384, 768), (100, 18944, 130),
-           (180, 300, 4000), (523, 7936, 164)]
+SINGLES = [(1, 512, 2048), (3, 700, 500), (8, 2000, 4096), (2, 5000, 200), (7, 19500, 500), (13, 20000, 100),
+           (16, 900, 4096), (32, 300, 1000), (30, 19000, 64), (64, 1000, 4096), (50, 19001, 96), (128, 384, 768),
+           (100, 18944, 130), (180, 300, 4000), (523, 7936, 164)]
 
 
 def choice(m, n, k, sms=SMS):
