@@ -183,6 +183,9 @@ typedef struct {
   int32_t turns;
 } sbc_mx_choice;
 int sbc_test_mx_plan(int64_t m, int64_t n, int64_t k, int32_t sms, sbc_mx_choice *out);
+/* sbc_test_mx_fault: as if a product on `device` had run out of a wait (a host
+ * store; nothing runs). */
+void sbc_test_mx_fault(int32_t device);
 int sbc_test_fault_mode(int mode);
 void sbc_test_withhold_tile(uint32_t job, uint64_t wait_limit_ns);
 
@@ -219,9 +222,9 @@ int sbc_mx_dequantize(const sbc_mx *q, void *out, int32_t dtype, int32_t transpo
 int sbc_mx_fuses_quantize(int64_t m, int64_t n, int64_t k);
 int sbc_mx_product(const sbc_mx *a, const void *x, int32_t x_dtype, int64_t x_stride, const sbc_mx *b, void *y,
                    int32_t dtype, int32_t after_quantize, void *stream);
-/* 2 once after a product whose bounded wait ran out (its output is
- * incomplete), else 0; -1 when the word could not be allocated. */
-int sbc_mx_take_fault(void);
+/* 2 once after a product on `device` whose bounded wait ran out (its output is
+ * incomplete), else 0. */
+int sbc_mx_take_fault(int32_t device);
 /* h = silu(gate) up over [rows, cols]; gate_q, up_q (mxint8, or both NULL)
  * keep the inputs in 8 bits. Rows are `*_stride` elements apart; h is dense. */
 int sbc_silu_mul(const void *gate, int64_t gate_stride, const void *up, int64_t up_stride, int32_t dtype, int64_t rows,

@@ -262,8 +262,9 @@ void sb_resources_free(sb_resources *resources);
  * columns adjacent. All calls are asynchronous on `stream` (a cudaStream_t of
  * the matrices' device), may be captured into a CUDA graph and leave the
  * caller's device current. A product whose bounded wait ran out (no such wait
- * runs out unless the device stalls for a second) is reported by the next
- * product as backend_failure. */
+ * runs out unless the device stalls for a second) is reported as backend_failure
+ * by sb_mx_status, or by the next product on its device, which is then not
+ * launched. */
 typedef struct {
   uint64_t codes;
   uint64_t scales;
@@ -290,6 +291,9 @@ int sb_mx_matmul(const sb_mx *a, const sb_mx *b, void *y, int32_t dtype, void *s
 int sb_mx_linear_workspace(int64_t rows, int64_t n, int64_t k, int32_t device, int64_t *bytes, sb_error *err);
 int sb_mx_linear(const void *x, int32_t x_dtype, int64_t rows, int64_t row_stride, const sb_mx *weight, void *y,
                  int32_t y_dtype, void *workspace, int64_t workspace_bytes, void *stream, sb_error *err);
+/* backend_failure, once, where a wait ran out in a product on `device` that has
+ * completed: replays of captured products too. Does not wait. */
+int sb_mx_status(int32_t device, sb_error *err);
 /* h [rows, cols] = silu(gate) up, dense; gate_q, up_q (mxint8, or both NULL)
  * keep the inputs for the backward call. */
 int sb_silu_mul(const void *gate, int64_t gate_stride, const void *up, int64_t up_stride, int32_t dtype, int64_t rows,

@@ -122,6 +122,7 @@ def lib():
         "sb_mx_quantize": (ctypes.c_int, [vp, i32, i64, i64, i64, mp, mp, vp, ep]),
         "sb_mx_dequantize": (ctypes.c_int, [mp, vp, i32, i32, vp, ep]),
         "sb_mx_matmul": (ctypes.c_int, [mp, mp, vp, i32, vp, ep]),
+        "sb_mx_status": (ctypes.c_int, [i32, ep]),
         "sb_mx_linear_workspace": (ctypes.c_int, [i64, i64, i64, i32, ctypes.POINTER(i64), ep]),
         "sb_mx_linear": (ctypes.c_int, [vp, i32, i64, i64, mp, vp, i32, vp, i64, vp, ep]),
         "sb_silu_mul": (ctypes.c_int, [vp, i64, vp, i64, i32, i64, i64, i32, vp, mp, mp, vp, ep]),
@@ -142,7 +143,7 @@ def cuda_layer():
     """The thin CUDA layer (libsb_cuda.so, include/sb_cuda.h), loaded by the
     runtime library; for its wait-limit setting and the test hooks that
     inject failures (``sbc_test_fault_mode``, ``sbc_test_withhold_tile``,
-    ``sbc_test_withhold_mx``) or tell the kernel choice (``sbc_test_mx_plan``)."""
+    ``sbc_test_withhold_mx``, ``sbc_test_mx_fault``) or tell the kernel choice (``sbc_test_mx_plan``)."""
     global _cuda
     if _cuda is not None:
         return _cuda
@@ -154,6 +155,8 @@ def cuda_layer():
     L.sbc_test_withhold_tile.argtypes = [ctypes.c_uint32, ctypes.c_uint64]
     L.sbc_test_withhold_mx.restype = None
     L.sbc_test_withhold_mx.argtypes = [ctypes.c_uint64]
+    L.sbc_test_mx_fault.restype = None
+    L.sbc_test_mx_fault.argtypes = [ctypes.c_int32]
     L.sbc_test_mx_plan.restype = ctypes.c_int
     L.sbc_test_mx_plan.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
                                    ctypes.POINTER(SbcMxChoice)]

@@ -27,6 +27,7 @@
 #include "mx_values.h"
 
 #include <atomic>
+#include <cstring>
 #include <mutex>
 #include <type_traits>
 
@@ -1015,23 +1016,44 @@ int launch_plan(const ProductArgs &a, const Plan &p, const sbc_mx *qa, const sbc
 /// Armed by sbc_test_withhold_mx: the wait limit of the next launch.
 std::atomic<uint64_t> g_withhold{0};
 
-/// The word in mapped pinned host memory that kernels set to 2 when a wait
-/// runs out: one for the process, allocated on first use.
+/// The words in mapped pinned host memory that kernels set to 2 when a wait
+/// runs out, one per device (64 bytes apart; devices from 63 on share the
+/// last), so that one device's stall says nothing of another's products.
+constexpr int kFaultWords = 64, kFaultPitch = 16;
+std::atomic<int32_t *> g_fault_words{nullptr};
+
+int32_t *fault_word_of(int32_t *words, int device) {
+  return words + kFaultPitch * (device < kFaultWords ? device : kFaultWords - 1);
+}
+
+/// The current device's word; allocated with the first product, NULL where that
+/// fails (the next product tries again).
 int32_t *fault_word() {
-  static int32_t *word = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    // legal while some stream is being captured
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    void *p = nullptr;
-    if (cudaHostAlloc(&p, 64, cudaHostAllocMapped | cudaHostAllocPortable) == cudaSuccess) {
-      word = static_cast<int32_t *>(p);
-      *word = 0;
+  static std::mutex lock;
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess)
+    return nullptr;
+  int32_t *words = g_fault_words.load(std::memory_order_acquire);
+  if (!words) {
+    const std::lock_guard<std::mutex> held(lock);
+    words = g_fault_words.load(std::memory_order_relaxed);
+    if (!words) {
+      // legal while some stream is being captured
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      void *p = nullptr;
+      const size_t bytes = kFaultWords * kFaultPitch * sizeof(int32_t);
+      if (cudaHostAlloc(&p, bytes, cudaHostAllocMapped | cudaHostAllocPortable) == cudaSuccess) {
+        words = static_cast<int32_t *>(p);
+        std::memset(words, 0, bytes);
+        g_fault_words.store(words, std::memory_order_release);
+      } else {
+        cudaGetLastError();
+      }
+      cudaThreadExchangeStreamCaptureMode(&mode);
     }
-    cudaThreadExchangeStreamCaptureMode(&mode);
-  });
-  return word;
+  }
+  return words ? fault_word_of(words, device) : nullptr;
 }
 
 } // namespace
@@ -1049,11 +1071,14 @@ int sbc_test_mx_plan(int64_t m, int64_t n, int64_t k, int32_t sms, sbc_mx_choice
   return 0;
 }
 
-int sbc_mx_take_fault(void) {
-  int32_t *w = fault_word();
-  if (!w)
-    return -1;
-  return __atomic_exchange_n(w, 0, __ATOMIC_RELAXED);
+int sbc_mx_take_fault(int32_t device) {
+  int32_t *words = g_fault_words.load(std::memory_order_acquire);
+  return words && device >= 0 ? __atomic_exchange_n(fault_word_of(words, device), 0, __ATOMIC_RELAXED) : 0;
+}
+
+void sbc_test_mx_fault(int32_t device) {
+  if (fault_word() && device >= 0)
+    __atomic_store_n(fault_word_of(g_fault_words.load(std::memory_order_acquire), device), 2, __ATOMIC_RELAXED);
 }
 
 int sbc_mx_fuses_quantize(int64_t m, int64_t n, int64_t k) {
@@ -1065,7 +1090,9 @@ int sbc_mx_product(const sbc_mx *a, const void *x, int32_t x_dtype, int64_t x_st
                    int32_t dtype, int32_t after_quantize, void *stream) {
   Plan p;
   int32_t *fault = fault_word();
-  if (!a || !b || !y || !fault || a->format != SBC_MXFP4 || b->format != SBC_MXFP4 || a->rows <= 0 || b->rows <= 0 ||
+  if (!fault)
+    return cudaErrorMemoryAllocation;
+  if (!a || !b || !y || a->format != SBC_MXFP4 || b->format != SBC_MXFP4 || a->rows <= 0 || b->rows <= 0 ||
       a->cols <= 0 || a->cols != b->cols || dtype < SBC_F32 || dtype > SBC_BF16 ||
       !plan_of(a->rows, b->rows, a->cols, sm_count(), &p) || (x && !p.fused) || (!x && !a->codes))
     return SBC_EINVAL;

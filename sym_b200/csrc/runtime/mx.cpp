@@ -83,13 +83,11 @@ int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 int64_t code_bytes(int64_t rows, int64_t cols) { return rows * ((cols + 31) / 32) * 16; }
 int64_t scale_bytes(int64_t rows, int64_t cols) { return (rows + 127) / 128 * ((cols + 127) / 128) * 512; }
 
-/// A wait that ran out in an earlier call's kernel is reported by the next
-/// call, as for the transfers with asynchronous completion.
-int earlier_fault(sb_error *err) {
-  const int f = sbc_mx_take_fault();
-  if (f < 0)
-    return fail(err, "backend_failure", "no pinned host memory for the fault word");
-  if (f)
+/// A wait that ran out in an earlier call's kernel is reported by the device's
+/// next product, as for the transfers with asynchronous completion, or on request
+/// (sb_mx_status).
+int earlier_fault(int32_t device, sb_error *err) {
+  if (sbc_mx_take_fault(device))
     return fail(err, "backend_failure",
                 "a bounded wait ran out in an earlier microscaled product; that product's output is incomplete");
   return 0;
@@ -159,9 +157,15 @@ int sb_mx_matmul(const sb_mx *a, const sb_mx *b, void *y, int32_t dtype, void *s
   OnDevice on(a->device);
   if (on.rc())
     return status(err, "set device", on.rc());
-  if (earlier_fault(err))
+  if (earlier_fault(a->device, err))
     return 1;
   return status(err, "matmul", sbc_mx_product(C(a), nullptr, 0, 0, C(b), y, dtype, 0, stream));
+}
+
+int sb_mx_status(int32_t device, sb_error *err) {
+  if (device < 0)
+    return fail(err, "invalid_view", "devices are numbered from 0");
+  return earlier_fault(device, err);
 }
 
 int sb_mx_linear_workspace(int64_t rows, int64_t n, int64_t k, int32_t device, int64_t *bytes, sb_error *err) {
@@ -187,7 +191,7 @@ int sb_mx_linear(const void *x, int32_t x_dtype, int64_t rows, int64_t row_strid
   OnDevice on(weight->device);
   if (on.rc())
     return status(err, "set device", on.rc());
-  if (earlier_fault(err))
+  if (earlier_fault(weight->device, err))
     return 1;
   const int64_t k = weight->cols;
   sbc_mx q{nullptr, nullptr, rows, k, SBC_MXFP4, weight->device};

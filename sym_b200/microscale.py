@@ -19,6 +19,7 @@ does so for mxfp4 weights, and ``linear`` multiplies with them directly.
 ``linear``                         values times an mxfp4 weight (serving), or times a
                                    float weight with all three products of a training
                                    step on mxfp4 operands
+``check``                          raises where a product did not complete
 ``silu_mul``                       silu(gate) * up, keeping gate and up in 8 bits for
                                    the backward pass
 
@@ -26,7 +27,8 @@ All calls run on the current stream of the tensors' device, allocate from
 torch's caching allocator only and can be captured into CUDA graphs (a backward
 pass, as torch asks, only while no eager graph of the same leaves is alive).
 They have no CPU execution. Wrong arguments raise ``ValueError`` or ``TypeError``; failures of the
-native layer raise ``pyreloc.TransferError``.
+native layer raise ``pyreloc.TransferError``. A product's waits are bounded; one
+that ran out is reported by the next product on its device, or by ``check``.
 
 Derivatives are those of reverse mode, once; codes carry none. Forward-mode
 tangents, ``vmap`` and second derivatives are refused. The kernels get addresses, which
@@ -398,6 +400,25 @@ def matmul(a, b, *, dtype=torch.bfloat16):
         raise ValueError(f"a [m, k] and b [n, k] need the same k: got {k} and {kb}")
     y = torch.empty((m, n), dtype=dtype, device=a.device)
     return _matmul_into(a.native, b.native, y) if m and n else y
+
+
+def check(device=None):
+    """Waits for the work of a device (default: the current one) and raises
+    ``pyreloc.TransferError`` where a product's bounded wait ran out since the
+    last report, so that its result is incomplete. The next eager product on the
+    device reports it too; this call is for those that none follows, replays of
+    captured graphs among them."""
+    if device is None or isinstance(device, int):
+        index = device
+    else:
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"microscaled operators run on CUDA devices: got {device}")
+        index = device.index
+    if index is None:
+        index = torch.cuda.current_device()
+    torch.cuda.synchronize(index)
+    _check(_lib().sb_mx_status(index, _scratch.ref))
 
 
 def _linear(x, w, dtype, shape):
