@@ -508,7 +508,8 @@ def linear(x, weight, weight_t=None, *, dtype=None):
     ``dx = Q(dy) weight_t^T``.
 
     ``weight`` a float tensor: training; x, weight and dy are quantised along the
-    axis that each product sums over, and the backward pass gives dx and dw."""
+    axis that each product sums over, and the backward pass gives dx and dw.
+    Where no gradient is asked for, the forms along k are made and dropped."""
     if _compiling():
         return _uncompiled(linear, x, weight, weight_t, dtype=dtype)
     _traceable("linear")
@@ -542,7 +543,10 @@ def linear(x, weight, weight_t=None, *, dtype=None):
         if _mx(weight_t, "weight_t", "mxfp4").shape != (k, n) or weight_t.device != x.device:
             raise ValueError(f"weight_t is [{k}, {n}] on {x.device}")
         return _FrozenLinear.apply(x, weight, weight_t, dtype)
-    return _TrainLinear.apply(x, weight, dtype)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad) or _jit_tracing():
+        return _TrainLinear.apply(x, weight, dtype)
+    # nothing to keep for a backward pass: the forms along k alone
+    return _linear(x, _quantize(weight, k, "mxfp4", True, False)[0], dtype, shape)
 
 
 class _SiluMul(torch.autograd.Function):
