@@ -251,8 +251,8 @@ void sb_resources_free(sb_resources *resources);
  *               codes: 16 bytes per block, the lower index in the lower half of
  *               a byte. scales: tiles of 128 rows x 4 blocks, 512 bytes, the
  *               tiles of 128 rows consecutive; row r, block b of a tile at byte
- *               16 (r mod 32) + 4 (r / 32) + b; absent blocks of a row's last
- *               tile hold 0.
+ *               16 (r mod 32) + 4 (r / 32) + b; absent blocks and rows of the
+ *               last tiles hold 0.
  *   mxint8 (1)  s = max(e, -120); k = rne(x 2^(6-s)), |k| <= 127.
  *               codes: 32 bytes per block; scales: row-major.
  * Rows are padded to whole blocks with zero codes. Codes and scales are device

@@ -73,6 +73,15 @@ __device__ __forceinline__ void quantize_part(const Raw8<DT> (&in)[V / 8], float
     *scales = static_cast<uint8_t>(exists ? byte : 0);
 }
 
+/// The words of a scale tile's rows past the matrix's last are 0: no product
+/// stores what they scale, but the same values have the same bytes. Thread t
+/// < 128 of the block that has the matrix's last row in this tile column.
+__device__ __forceinline__ void clear_absent_rows(uint8_t *scales, int64_t rows, int64_t tc, int64_t quads) {
+  const int64_t r = ((rows - 1) & ~int64_t{127}) + threadIdx.x;
+  if (threadIdx.x < 128 && r >= rows)
+    *reinterpret_cast<uint32_t *>(scales + scale_word(r, tc, quads)) = 0;
+}
+
 /// The parts of a block's rows from r0 on, whose starts have no alignment.
 template <int DT, int UNITS>
 __device__ __forceinline__ void load_ragged(Part<DT> (&in)[UNITS], const QuantizeArgs &a, int64_t r0, int64_t c0) {
@@ -135,6 +144,8 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize(const __grid_constant_
     quantize_part<DT, FMT, V>(in[i].raw, in[i].block_top(), codes + i * code_step, scales + scale_step,
                               row_exists && exists, row_exists);
   }
+  if (FMT == SBC_MXFP4 && static_cast<int64_t>(tr + 1) * (kUnits * kStride) >= a.rows)
+    clear_absent_rows(a.scales, a.rows, tc, quads_of(a.cols));
 }
 
 /// Blocks along the rows, and with ROWS along the columns too, from one read:
@@ -180,6 +191,8 @@ __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 1 : VEC ? 4 : 3) k_m
                                       row_scales + (i * kStride / 32) * 4 + (i * kStride % 32) * 16,
                                       row < here && c < row_blocks * kBlock, row < here);
   }
+  if (ROWS && here < kTile)
+    clear_absent_rows(a.scales, a.rows, tc, quads_of(a.cols));
   __syncthreads();
   // Blocks along the rows: a thread takes 32 rows of two neighbouring 16-bit
   // columns, or of two 32-bit columns 64 apart, so that the lanes of a warp
@@ -232,11 +245,10 @@ __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 1 : VEC ? 4 : 3) k_m
       *reinterpret_cast<uint4 *>(a.codes_t + (c0 + col) * blocks * 16 + (r0 / 32 + rb) * 16) =
           codes[col * 4 + (rb ^ (col >> 1 & 3))];
   }
-  if (t < 128) { // rows of the scale tile past the last column stay as they were
+  if (t < 128) { // 0 for the scale tile's rows past the last column
     const int col = (t >> 2) + 32 * (t & 3);
-    if (c0 + col < a.cols)
-      *reinterpret_cast<uint32_t *>(a.scales_t + scale_word(c0 + col, tr, quads)) =
-          reinterpret_cast<const uint32_t *>(scales)[t];
+    *reinterpret_cast<uint32_t *>(a.scales_t + scale_word(c0 + col, tr, quads)) =
+        c0 + col < a.cols ? reinterpret_cast<const uint32_t *>(scales)[t] : 0;
   }
 }
 
