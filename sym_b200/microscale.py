@@ -137,7 +137,13 @@ class MxTensor:
     and uint8 ``scales`` (flat, in the format's order).
 
     The constructor takes tensors that already have that layout, without a
-    copy; ``from_rows`` takes row-major scales, as checkpoints hold them. A
+    copy; ``from_rows`` takes row-major scales, as checkpoints hold them, and
+    pads them. Products take 64 values of a row at a time and trust the padding:
+    codes past a row's end are 0, and so are, in mxfp4's tiles, the scale bytes
+    that a row's last tile has for blocks that do not exist (what it has for
+    rows past the last is not read). Of tensors in host memory the constructor
+    checks those bytes; on a device that would have to wait for the data, so what
+    comes from elsewhere is best brought as host tensors or by ``from_rows``. A
     matrix keeps its tensors; they are not exchanged for others (``native``
     holds their addresses), but copies and pickles are made from them."""
 
@@ -164,6 +170,11 @@ class MxTensor:
         if scales.numel() != _scale_bytes(rows, cols, format) or not scales.is_contiguous():
             raise ValueError(f"{format} scales of [{rows}, {cols}] are {_scale_bytes(rows, cols, format)} "
                              "contiguous bytes")
+        blocks = _blocks(cols)
+        if format == "mxfp4" and scales.device.type == "cpu" and blocks % 4:
+            last = scales.view(-(-rows // 128), -(-blocks // 4), 32, 4, 4)[:, -1].transpose(1, 2)
+            if last.reshape(-1, 4)[:rows, blocks % 4:].any():
+                raise ValueError("scale bytes of blocks that do not exist are 0 in a row's last tile")
         self._codes, self._scales, self._shape, self._format = codes, scales, (rows, cols), format
         self._native = None
         if codes.is_cuda and rows:
