@@ -235,6 +235,8 @@ class MxTensor:
 
 def _matrix(x, cols):
     """x [..., cols] as a matrix whose columns are adjacent: (tensor, rows, cols, row stride)."""
+    if x.is_neg():  # a view whose memory holds the negated values
+        x = x.resolve_neg()
     if x.is_contiguous():
         return x, x.numel() // cols, cols, cols
     if x.dim() != 2:
