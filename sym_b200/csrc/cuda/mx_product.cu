@@ -43,6 +43,10 @@ constexpr int kThreads = 192;     // warp 0 loads, warp 1 multiplies, warps 2-5 
 constexpr int kMaxSplit = 8;      // portable cluster size
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kUnits = 4;         // FUSED: units of 8 values of A in flight per thread
+// The wait limit is for one step, whose copies or products are awaited. The
+// storing warps await all steps of a tile: they add this for each, five times
+// what a step takes with every SM streaming at the memory's rate.
+constexpr uint64_t kStepNs = 8000;
 
 struct ProductArgs {
   CUtensorMap map_a, map_b; // codes [rows, bytes], boxes of NT (128) rows x 128 bytes, 128-byte swizzle
@@ -379,7 +383,7 @@ __global__ void __launch_bounds__(kThreads) k_mx_product(const __grid_constant__
     const int quarter = warp & 3; // the lanes of tensor memory that this warp may read
     const int row = quarter * 32 + lane;
     const uint32_t acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    if (!warp_wait(&ready, 0, a.wait_ns))
+    if (!warp_wait(&ready, 0, a.wait_ns + (ks1 - ks0) * kStepNs))
       *a.fault = 2;
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     // The part's sums as [cols][128] in the stages, all of which have been read.
@@ -695,7 +699,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_mx_product_pair(const __gri
       const uint32_t buf = turn % S::kBufs, use = turn / S::kBufs;
       uint32_t tb, ta;
       pair_tile(a, i, tb, ta);
-      if (!warp_wait(&ready[buf], use & 1, a.wait_ns)) {
+      if (!warp_wait(&ready[buf], use & 1, a.wait_ns + a.steps * kStepNs)) {
         *a.fault = 2;
         break;
       }
