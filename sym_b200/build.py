@@ -92,6 +92,8 @@ def build(force: bool = False, verbose: bool = False) -> None:
             objects.append(obj)
             if force or not same or _stale(obj, _dependencies(obj.with_suffix(".d"), [src] + HEADERS)):
                 todo.append([*cmd, "-MD", "-MF", obj.with_suffix(".d"), "-c", src, "-o", obj])
+        if not same:  # until every object is made with this line, none is known to be
+            recipe.unlink(missing_ok=True)
         with ThreadPoolExecutor(max_workers=max(1, min(len(todo), os.cpu_count() or 1))) as pool:
             list(pool.map(lambda c: _run(c, verbose), todo))
         recipe.write_text(line)
