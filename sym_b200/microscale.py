@@ -40,6 +40,7 @@ calls as they are, between its graphs.
 from __future__ import annotations
 
 import ctypes
+import operator
 import threading
 from functools import lru_cache
 
@@ -157,7 +158,9 @@ class MxTensor:
     def __init__(self, codes, scales, shape, format="mxfp4"):
         if format not in FORMATS:
             raise ValueError(f"format must be one of {sorted(FORMATS)}")
-        rows, cols = shape
+        rows, cols = map(operator.index, shape)
+        if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
+            raise TypeError("codes and scales are uint8 tensors")
         if rows < 0 or cols < 1:
             raise ValueError("a microscaled matrix has at least one column")
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
@@ -201,6 +204,9 @@ class MxTensor:
     @classmethod
     def from_rows(cls, codes, row_scales, cols, format="mxfp4"):
         """From codes and row-major scales ``[rows, blocks]``."""
+        if not isinstance(codes, torch.Tensor) or not isinstance(row_scales, torch.Tensor):
+            raise TypeError("codes and row_scales are uint8 tensors")
+        cols = operator.index(cols)
         rows, blocks = row_scales.shape
         if blocks != _blocks(cols):
             raise ValueError(f"rows of {cols} values have {_blocks(cols)} scales")

@@ -45,6 +45,23 @@ def test_scales_of_blocks_that_do_not_exist_are_refused(rows, cols):
     mx.MxTensor(torch.zeros(0, blocks * 16, dtype=torch.uint8), torch.zeros(0, dtype=torch.uint8), (0, cols))
 
 
+def test_what_is_no_matrix_is_refused_as_such():
+    codes, scales, rows = (torch.zeros(*s, dtype=torch.uint8) for s in ((4, 32), (512,), (4, 2)))
+    for call in (lambda: mx.MxTensor(None, scales, (4, 64)), lambda: mx.MxTensor(codes, [0] * 512, (4, 64)),
+                 lambda: mx.MxTensor(codes, scales, (4.0, 64)), lambda: mx.MxTensor(codes, scales, (4, "64")),
+                 lambda: mx.MxTensor(codes, scales, 256), lambda: mx.MxTensor.from_rows(None, rows, 64),
+                 lambda: mx.MxTensor.from_rows(codes, [[0, 0]] * 4, 64), lambda: mx.MxTensor.from_rows(codes, rows, 64.0)):
+        with pytest.raises(TypeError):
+            call()
+    for call in (lambda: mx.MxTensor(codes, scales, (4,)), lambda: mx.MxTensor(codes, scales, (4, 64, 1)),
+                 lambda: mx.MxTensor.from_rows(codes, rows[0], 64), lambda: mx.MxTensor.from_rows(codes, rows, 0),
+                 lambda: mx.MxTensor.from_rows(codes, rows, 64, "fp4")):
+        with pytest.raises(ValueError):
+            call()
+    q = mx.MxTensor.from_rows(codes, rows, torch.tensor(64))
+    assert q.shape == (4, 64) and all(type(n) is int for n in q.shape)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k", [(1, 300, 2050), (8, 2000, 4110), (13, 20000, 65), (50, 19001, 70), (100, 300, 800),
                                    (180, 300, 4110), (163, 768, 130), (777, 11009, 2080), (1347, 9703, 66)])
