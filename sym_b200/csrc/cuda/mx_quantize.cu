@@ -9,12 +9,12 @@
 //
 // Measured (8192 x 8192, captured back to back; bytes of the task over time):
 //   rows, f16 26.2 us = 6.5 TB/s, f32 45.3 us = 6.7; both directions in one
-//   read, f16 40.1 us = 5.1, f32 68.5 us = 5.0 (the issue of the second
+//   read, f16 39.1 us = 5.3, f32 64.7 us = 5.3 (the issue of the second
 //   direction's instructions, 66 % busy); across alone, f16 34.6 us = 4.9;
 //   back to values, f16 26.3 us = 6.5, f32 47.7 us = 6.4, transposed f16
 //   30.2 us = 5.6, f32 56 us = 5.4. [28672, 8192] to [in, out]: f16 111 us = 5.4,
 //   f32 184 us = 5.8.
-//   Rows of 8191 columns (through shared memory per warp): f16 39.4, 59.8 and,
+//   Rows of 8191 columns (through shared memory per warp): f16 39.9, 61 and,
 //   back, 36.7 us; each lane by itself 53, 80 and 196.
 #include "barriers.h"
 #include "mx_values.h"
@@ -75,7 +75,11 @@ __device__ __forceinline__ void quantize_part(const Raw8<DT> (&in)[V / 8], float
 
 /// The words of a scale tile's rows past the matrix's last are 0: no product
 /// stores what they scale, but the same values have the same bytes. Thread t
-/// < 128 of the block that has the matrix's last row in this tile column.
+/// < 128 of the block that has the matrix's last row in this tile column. Where
+/// the call stands decides what the compiler keeps in registers. Both directions,
+/// rows off 16-byte boundaries: first (8192 x 8191 f16 61 us; last 73, with
+/// spills); aligned rows: last (8192 x 8192 f32 64.7 us; first 70.2). One
+/// direction: last (8192 x 8192 f16 26.2 us; first 26.7).
 __device__ __forceinline__ void clear_absent_rows(uint8_t *scales, int64_t rows, int64_t tc, int64_t quads) {
   const int64_t r = ((rows - 1) & ~int64_t{127}) + threadIdx.x;
   if (threadIdx.x < 128 && r >= rows)
@@ -151,8 +155,8 @@ __global__ void __launch_bounds__(kThreads) k_mx_quantize(const __grid_constant_
 /// Blocks along the rows, and with ROWS along the columns too, from one read:
 /// a tile of 128 x 128 values. 16-bit values: four blocks an SM (64 registers;
 /// across alone 34.6 us against 40.6 for 8192 x 8192). 32-bit values: as many
-/// registers as hold all of a thread's loads (116, two blocks an SM; three
-/// blocks took 79 us for both directions, two 68).
+/// registers as hold all of a thread's loads (124, two blocks an SM; three
+/// blocks took 79 us for both directions, two 65).
 template <int DT, bool ROWS, bool VEC>
 __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 1 : VEC ? 4 : 3) k_mx_quantize_across(const __grid_constant__ QuantizeArgs a) {
   using T = typename Value<DT>::T;
@@ -170,6 +174,8 @@ __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 1 : VEC ? 4 : 3) k_m
   uint4 *codes = smem + kTile * kTile * sizeof(T) / 16;            // [128 columns][4]
   uint8_t *scales = reinterpret_cast<uint8_t *>(codes + kTile * 4); // [512]
   const int64_t row_blocks = blocks_of(a.cols);
+  if (!VEC && ROWS && here < kTile)
+    clear_absent_rows(a.scales, a.rows, tc, quads_of(a.cols));
   uint8_t *row_codes = a.codes + (r0 + row0) * row_blocks * 16 + c / 2;
   uint8_t *row_scales = a.scales + scale_word(r0 + row0, tc, quads_of(a.cols)) + c8 / 32;
   Part<DT> in[kUnits];
@@ -191,8 +197,6 @@ __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 1 : VEC ? 4 : 3) k_m
                                       row_scales + (i * kStride / 32) * 4 + (i * kStride % 32) * 16,
                                       row < here && c < row_blocks * kBlock, row < here);
   }
-  if (ROWS && here < kTile)
-    clear_absent_rows(a.scales, a.rows, tc, quads_of(a.cols));
   __syncthreads();
   // Blocks along the rows: a thread takes 32 rows of two neighbouring 16-bit
   // columns, or of two 32-bit columns 64 apart, so that the lanes of a warp
@@ -250,6 +254,8 @@ __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 1 : VEC ? 4 : 3) k_m
     *reinterpret_cast<uint32_t *>(a.scales_t + scale_word(c0 + col, tr, quads)) =
         c0 + col < a.cols ? reinterpret_cast<const uint32_t *>(scales)[t] : 0;
   }
+  if (VEC && ROWS && here < kTile)
+    clear_absent_rows(a.scales, a.rows, tc, quads_of(a.cols));
 }
 
 struct DequantizeArgs {
@@ -395,7 +401,8 @@ __global__ void __launch_bounds__(kThreads, DT == SBC_F32 ? 3 : 4) k_mx_dequanti
     if (VEC && (have <= 0 || c0 + 8 * c >= a.cols))
       continue;
     // Two columns at a time from the codes' 16-bit values, which keeps the
-    // registers of four blocks to an SM. What was staged for rows past the end
+    // registers of four blocks to an SM (16-bit values: 64, at the price of 44
+    // bytes of spills). What was staged for rows past the end
     // is never stored.
     uint32_t h[8][4];
     float scale[8];

@@ -92,12 +92,11 @@ def _uncompiled(call, *args, **kwargs):
 def _traceable(call, jit=False):
     """Refuses a call whose result a recorder would keep as the allocation alone:
     under make_fx, and where the call is no autograd function (``jit``) under
-    torch.jit.trace."""
-    if _modes() or _key_included(_PRE_DISPATCH):
-        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    torch.jit.trace. Called where some dispatch mode or a tracer is at work."""
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
 
-        if get_proxy_mode() is not None:
-            raise NotImplementedError(f"{call} cannot be recorded by make_fx: its kernels take addresses")
+    if get_proxy_mode() is not None:
+        raise NotImplementedError(f"{call} cannot be recorded by make_fx: its kernels take addresses")
     if jit and _jit_tracing():
         raise NotImplementedError(f"{call} cannot be recorded by torch.jit.trace: its kernels take addresses")
 
@@ -165,26 +164,27 @@ class MxTensor:
             raise ValueError("a microscaled matrix has at least one column")
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError("codes and scales are uint8 tensors")
-        if codes.device != scales.device:
+        on_cuda = codes.is_cuda
+        if codes.get_device() != scales.get_device() or not on_cuda and codes.device != scales.device:
             raise ValueError("codes and scales live on different devices")
-        if tuple(codes.shape) != (rows, _blocks(cols) * _CODE_BYTES[format]) or not codes.is_contiguous():
-            raise ValueError(f"{format} codes of [{rows}, {cols}] are a contiguous "
-                             f"[{rows}, {_blocks(cols) * _CODE_BYTES[format]}] tensor")
-        if scales.numel() != _scale_bytes(rows, cols, format) or not scales.is_contiguous():
-            raise ValueError(f"{format} scales of [{rows}, {cols}] are {_scale_bytes(rows, cols, format)} "
-                             "contiguous bytes")
         blocks = _blocks(cols)
-        if format == "mxfp4" and scales.device.type == "cpu" and blocks % 4:
+        width = blocks * _CODE_BYTES[format]
+        if codes.shape != (rows, width) or not codes.is_contiguous():
+            raise ValueError(f"{format} codes of [{rows}, {cols}] are a contiguous [{rows}, {width}] tensor")
+        held = _scale_bytes(rows, cols, format)
+        if scales.numel() != held or not scales.is_contiguous():
+            raise ValueError(f"{format} scales of [{rows}, {cols}] are {held} contiguous bytes")
+        self._codes, self._scales, self._shape, self._format = codes, scales, (rows, cols), format
+        self._native = None
+        if on_cuda and rows:
+            at, scales_at = codes.data_ptr(), scales.data_ptr()
+            if at % 16 or scales_at % 16:
+                raise ValueError("codes and scales start on 16-byte boundaries")
+            self._native = _native.SbMx(at, scales_at, rows, cols, FORMATS[format], codes.get_device())
+        elif blocks % 4 and format == "mxfp4" and codes.device.type == "cpu":
             last = scales.view(-(-rows // 128), -(-blocks // 4), 32, 4, 4)[:, -1].transpose(1, 2)
             if last.reshape(-1, 4)[:rows, blocks % 4:].any():
                 raise ValueError("scale bytes of blocks that do not exist are 0 in a row's last tile")
-        self._codes, self._scales, self._shape, self._format = codes, scales, (rows, cols), format
-        self._native = None
-        if codes.is_cuda and rows:
-            if codes.data_ptr() % 16 or scales.data_ptr() % 16:
-                raise ValueError("codes and scales start on 16-byte boundaries")
-            self._native = _native.SbMx(codes.data_ptr(), scales.data_ptr(), rows, cols, FORMATS[format],
-                                       codes.device.index)
 
     @classmethod
     def _empty(cls, like, rows, cols, format="mxfp4"):
@@ -270,15 +270,14 @@ def _values(x, name):
 def _mx(q, name, format=None):
     if type(q) is not MxTensor:
         raise TypeError(f"{name} is an MxTensor")
-    if not q.codes.is_cuda:
+    if not q._codes.is_cuda:
         raise ValueError(f"{name} is on {q.device}: microscaled operators run on CUDA devices")
-    if format is not None and q.format != format:
-        raise ValueError(f"{name} is {q.format}: {format} is needed")
+    if format is not None and q._format != format:
+        raise ValueError(f"{name} is {q._format}: {format} is needed")
     return q
 
 
-def _result(dtype, default):
-    dtype = default if dtype is None else dtype
+def _result(dtype):
     if dtype not in _DTYPES:
         raise TypeError("results are float32, float16 or bfloat16")
     return dtype
@@ -348,7 +347,8 @@ def quantize(x, format="mxfp4", *, along=-1):
     the first axis."""
     if _compiling():
         return _uncompiled(quantize, x, format, along=along)
-    _traceable("quantize", jit=True)
+    if _modes() or _key_included(_PRE_DISPATCH) or _jit_tracing():
+        _traceable("quantize", jit=True)
     shape = _values(x, "x")
     if format not in FORMATS:
         raise ValueError(f"format must be one of {sorted(FORMATS)}")
@@ -371,7 +371,8 @@ def quantize_both(x):
     quantize(x, along=0))``, what a training step's products take."""
     if _compiling():
         return _uncompiled(quantize_both, x)
-    _traceable("quantize_both", jit=True)
+    if _modes() or _key_included(_PRE_DISPATCH) or _jit_tracing():
+        _traceable("quantize_both", jit=True)
     shape = _values(x, "x")
     if len(shape) != 2 or shape[0] == 0:
         raise ValueError("quantize_both takes a matrix with at least one row")
@@ -384,9 +385,10 @@ def dequantize(q, dtype=torch.float16, *, transpose=False):
     product ``x @ w`` takes."""
     if _compiling():
         return _uncompiled(dequantize, q, dtype, transpose=transpose)
-    _traceable("dequantize", jit=True)
+    if _modes() or _key_included(_PRE_DISPATCH) or _jit_tracing():
+        _traceable("dequantize", jit=True)
     _mx(q, "q")
-    dtype = _result(dtype, None)
+    dtype = _result(dtype)
     if transpose and q.format != "mxfp4":
         raise ValueError("transpose is defined for mxfp4")
     rows, cols = q.shape
@@ -409,15 +411,16 @@ def matmul(a, b, *, dtype=torch.bfloat16):
     32 bits and rounded once to ``dtype``."""
     if _compiling():
         return _uncompiled(matmul, a, b, dtype=dtype)
-    _traceable("matmul", jit=True)
+    if _modes() or _key_included(_PRE_DISPATCH) or _jit_tracing():
+        _traceable("matmul", jit=True)
     _mx(a, "a", "mxfp4"), _mx(b, "b", "mxfp4")
-    dtype = _result(dtype, None)
-    if a.device != b.device:
+    dtype = _result(dtype)
+    if a.get_device() != b.get_device():
         raise ValueError("a and b live on different devices")
     (m, k), (n, kb) = a.shape, b.shape
     if k != kb:
         raise ValueError(f"a [m, k] and b [n, k] need the same k: got {k} and {kb}")
-    y = torch.empty((m, n), dtype=dtype, device=a.device)
+    y = a._codes.new_empty((m, n), dtype=dtype)
     return _matmul_into(a.native, b.native, y) if m and n else y
 
 
@@ -531,15 +534,15 @@ def linear(x, weight, weight_t=None, *, dtype=None):
     Where no gradient is asked for, the forms along k are made and dropped."""
     if _compiling():
         return _uncompiled(linear, x, weight, weight_t, dtype=dtype)
-    _traceable("linear")
+    if _modes() or _key_included(_PRE_DISPATCH):
+        _traceable("linear")
     if _forward_ad._current_level >= 0:
         _no_tangents("linear", x, weight)
     shape = _values(x, "x")
-    dtype = _result(dtype, x.dtype)
+    dtype = x.dtype if dtype is None else _result(dtype)
     frozen = type(weight) is MxTensor
     if frozen:
-        _mx(weight, "weight", "mxfp4")
-        n, k = weight._shape
+        n, k = _mx(weight, "weight", "mxfp4")._shape
     elif weight_t is not None:
         raise ValueError("weight_t goes with an MxTensor weight")
     else:
@@ -620,7 +623,8 @@ def silu_mul(gate, up=None):
     The result itself is computed from the inputs."""
     if _compiling():
         return _uncompiled(silu_mul, gate, up)
-    _traceable("silu_mul")
+    if _modes() or _key_included(_PRE_DISPATCH):
+        _traceable("silu_mul")
     if _forward_ad._current_level >= 0:
         _no_tangents("silu_mul", gate, up)
     shape = _values(gate, "gate")
