@@ -324,6 +324,8 @@ def _differentiable_once(backward):
     def run(ctx, *grads):
         if _compiling():
             return _uncompiled(run, ctx, *grads)
+        if _modes() or _key_included(_PRE_DISPATCH):
+            _traceable("a backward pass")
         return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
     return run

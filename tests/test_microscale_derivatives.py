@@ -47,6 +47,15 @@ def test_tracing_of_calls_that_are_no_autograd_functions_is_refused():
             torch.jit.trace(call, (x,), check_trace=False)
 
 
+def test_make_fx_of_a_backward_pass_is_refused():
+    """Also where the forward pass was not recorded."""
+    dy = torch.ones(2, 64)
+    for function in (mx._FrozenLinear, mx._TrainLinear, mx._SiluMul):
+        for pre_dispatch in (False, True):
+            with pytest.raises(NotImplementedError, match="make_fx"):
+                make_fx(lambda dy: function.backward(None, dy), pre_dispatch=pre_dispatch)(dy)
+
+
 def test_other_dispatch_modes_are_no_recorders():
     from torch.utils.flop_counter import FlopCounterMode
 
@@ -98,6 +107,17 @@ def test_forward_mode_and_transforms_on_the_gpu():
         for mode in ("real", "fake", "symbolic"):
             with pytest.raises((RuntimeError, NotImplementedError)):
                 make_fx(call, tracing_mode=mode)(x)
+
+
+@pytest.mark.gpu
+def test_recorded_backward_passes_on_the_gpu():
+    x, w = tensor(5, 64).requires_grad_(), tensor(96, 64, seed=1)
+    q, qt = mx.quantize_both(w)
+    for y in (mx.linear(x, q, qt), mx.linear(x, w), mx.silu_mul(x)):
+        dy = torch.ones_like(y)
+        with pytest.raises(NotImplementedError):
+            make_fx(lambda dy: torch.autograd.grad(y, x, dy, retain_graph=True)[0])(dy)
+        assert torch.autograd.grad(y, x, dy)[0].isfinite().all()
 
 
 @pytest.mark.gpu
