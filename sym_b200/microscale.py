@@ -326,6 +326,8 @@ def _differentiable_once(backward):
             return _uncompiled(run, ctx, *grads)
         if _modes() or _key_included(_PRE_DISPATCH):
             _traceable("a backward pass")
+        if _forward_ad._current_level >= 0:
+            _no_tangents("a backward pass", *grads)
         return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
     return run

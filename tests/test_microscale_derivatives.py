@@ -56,6 +56,15 @@ def test_make_fx_of_a_backward_pass_is_refused():
                 make_fx(lambda dy: function.backward(None, dy), pre_dispatch=pre_dispatch)(dy)
 
 
+def test_tangents_of_incoming_gradients_are_refused():
+    dy = torch.ones(2, 64)
+    with fw.dual_level():
+        dual = fw.make_dual(dy, dy)
+        for function in (mx._FrozenLinear, mx._TrainLinear, mx._SiluMul):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                function.backward(None, dual)
+
+
 def test_other_dispatch_modes_are_no_recorders():
     from torch.utils.flop_counter import FlopCounterMode
 
@@ -117,6 +126,9 @@ def test_recorded_backward_passes_on_the_gpu():
         dy = torch.ones_like(y)
         with pytest.raises(NotImplementedError):
             make_fx(lambda dy: torch.autograd.grad(y, x, dy, retain_graph=True)[0])(dy)
+        with fw.dual_level():
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(y, x, fw.make_dual(dy, dy), retain_graph=True)
         assert torch.autograd.grad(y, x, dy)[0].isfinite().all()
 
 
